@@ -78,6 +78,10 @@ enum { EHIP_KV_F32 = 0, EHIP_KV_BF16 = 1, EHIP_KV_INT8 = 2, EHIP_KV_FP8 = 3 };
 /* Weight storage of the packed linear layer (the reference's PackedLinear
  * weight dtypes kFloat32 / kBFloat16 / kFloat16, src/model/packed_linear.h:31-36). */
 enum { EHIP_WEIGHT_F32 = 0, EHIP_WEIGHT_BF16 = 1, EHIP_WEIGHT_F16 = 2 };
+/* Activations of the gated feed-forward block: SiLU x / (1 + exp(-x)), GELU
+ * x (1 + erf(x / sqrt 2)) / 2, and GELU with tanh(sqrt(2 / pi) (x + 0.044715 x^3))
+ * in erf's place. */
+enum { EHIP_ACT_SILU = 0, EHIP_ACT_GELU = 1, EHIP_ACT_GELU_TANH = 2 };
 
 typedef struct ehip_ctx ehip_ctx;
 
@@ -252,6 +256,66 @@ int ehip_pack_weight_panels(ehip_ctx* ctx, const void* d_w, int32_t weight_dtype
  * owns). d_bias may be null. */
 int ehip_packed_gemm(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k, const void* d_wp,
                      int32_t weight_dtype, int64_t n, const float* d_bias, float* d_y);
+
+/* The gated feed-forward block over packed weights: both projections of x, the
+ * activation and the product in one kernel,
+ *   y[m, n] = act(x Wg^T + bias_gate) * (x Wu^T + bias_up).
+ * x, biases, y fp32; d_wp_gate and d_wp_up are two weights [n, k] of one type as
+ * ehip_pack_weight_panels lays them out (16-byte aligned). The sums are those of
+ * ehip_packed_gemm, in the same precision; results are deterministic. Biases may
+ * be null; m, k, n in [1, 2^21]; y may not overlap an operand. */
+int ehip_packed_gated_gemm(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k,
+                           const void* d_wp_gate, const void* d_wp_up, int32_t weight_dtype,
+                           int64_t n, const float* d_bias_gate, const float* d_bias_up,
+                           int32_t activation, float* d_y);
+
+/* ------------------------------------------ microscaled 4-bit (MXFP4) -----
+ * The OCP microscaling format with E2M1 elements: blocks of 32 consecutive k of
+ * one row (the last one may be shorter), each with a scale byte s that stands
+ * for 2^(s - 127) (255: NaN) and codes for 0, .5, 1, 1.5, 2, 3, 4, 6 and their
+ * negatives; value = code * scale. The matrices of the calls below are in
+ * panels of 16 rows, with k tiles of 128 (4 blocks) and groups of 4 tiles:
+ *   codes  [ceil(rows/16)][ceil(k/128)][64][16] bytes: entry 16 g + r of a tile
+ *          holds block g of panel row r, element 2i in the low half of byte i;
+ *   scales [ceil(rows/16)][ceil(k/512)][64][4] bytes: entry 16 g + r, byte j is
+ *          the scale of row r's block g in the group's tile j;
+ * zero bytes past the rows and the blocks. Codes are 16-byte aligned, scales 4.
+ * Rows and k in [1, 2^21]. No counterpart in the reference, whose weights end at
+ * 16 bits (src/model/packed_linear.h:31-36). */
+/* Bytes of a matrix's two arrays (host only; either pointer may be NULL). */
+int ehip_mxfp4_panel_bytes(int64_t rows, int64_t k, int64_t* codes_out, int64_t* scales_out);
+/* d_x [rows, k], contiguous, of type dtype (EHIP_WEIGHT_F32, _BF16 or _F16), in
+ * panels. A block's scale is 2^(floor(log2 max|x|) - 2), at least 2^-127 (also
+ * for a block of zeros); codes are x / scale rounded to nearest even, 6 at most
+ * in magnitude. A block with an infinity or a NaN gets the NaN scale. */
+int ehip_mxfp4_quantize(ehip_ctx* ctx, const void* d_x, int32_t dtype, int64_t rows, int64_t k,
+                        void* d_codes, void* d_scales);
+/* A matrix as checkpoints hold it, codes [rows, ceil(k/32), 16 bytes] and scales
+ * [rows, ceil(k/32)], in panels (a permutation; codes past k become zeros). */
+int ehip_mxfp4_pack(ehip_ctx* ctx, const uint8_t* d_row_codes, const uint8_t* d_row_scales,
+                    int64_t rows, int64_t k, void* d_codes, void* d_scales);
+/* The values of panels, fp32 [rows, k] (past fp32's largest: infinite). */
+int ehip_mxfp4_dequantize(ehip_ctx* ctx, const void* d_codes, const void* d_scales, int64_t rows,
+                          int64_t k, float* d_y);
+/* y[m, n] = x W^T (+ bias[n]) over panels of x [m, k] and W [n, k]: exact
+ * products, fp32 sums in a fixed order, bias added after them (may be null).
+ * For an x that several weights share; ehip_mxfp4_linear otherwise. */
+int ehip_mxfp4_gemm(ehip_ctx* ctx, const void* d_x_codes, const void* d_x_scales, int64_t m,
+                    int64_t k, const void* d_w_codes, const void* d_w_scales, int64_t n,
+                    const float* d_bias, float* d_y);
+/* The packed linear layer with an MXFP4 weight: x [m, k] fp32 is quantised as
+ * ehip_mxfp4_quantize does it, into a workspace the context owns, then
+ * multiplied as by ehip_mxfp4_gemm. */
+int ehip_mxfp4_linear(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k,
+                      const void* d_w_codes, const void* d_w_scales, int64_t n,
+                      const float* d_bias, float* d_y);
+/* The gated feed-forward block with MXFP4 weights, x quantised likewise:
+ * y[m, n] = act(x Wg^T + bias_gate) * (x Wu^T + bias_up). */
+int ehip_mxfp4_gated_linear(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k,
+                            const void* d_gate_codes, const void* d_gate_scales,
+                            const void* d_up_codes, const void* d_up_scales, int64_t n,
+                            const float* d_bias_gate, const float* d_bias_up, int32_t activation,
+                            float* d_y);
 
 /* kernels::PrefillAttentionVarlenF32 (src/kernels/attention.h:221-227), in the
  * reference's argument order: sequence b's query rows are [cu_seqlens[b],

@@ -35,9 +35,14 @@ struct ehip_ctx {
   // Split-KV partials (max, sum, unnormalised output per split).
   float* d_part = nullptr;
   size_t d_part_bytes = 0;
-  // Split-k partial sums of the packed linear layer.
+  // Workspace of the linear layers: x's planes or MXFP4 panels, split-k
+  // partial sums. A captured graph keeps its address, so one that a capture has
+  // used is retired, not freed, when a larger one takes its place.
   float* d_gemm = nullptr;
   size_t d_gemm_bytes = 0;
+  bool gemm_captured = false;
+  void* retired[64] = {};  // each growth is half as much again: 64 pass any memory
+  int n_retired = 0;
   int cus = 256;  // compute units of the device
   int32_t* d_err = nullptr;
   // Item-queue counters of the persistent decode kernel, in the error page
@@ -109,6 +114,35 @@ int EnsureWorkspace(ehip_ctx* ctx, const ehip_geometry& g, const Plan& plan) {
     EHIP_HIP(ctx, hipMalloc(&ctx->d_part, bytes));
     ctx->d_part_bytes = bytes;
   }
+  return EHIP_OK;
+}
+
+// Grows the linear layers' workspace to `need` bytes. It cannot grow while the
+// stream is being captured.
+int EnsureGemmWorkspace(ehip_ctx* ctx, size_t need) {
+  if (need == 0) return EHIP_OK;
+  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+  EHIP_HIP(ctx, hipStreamIsCapturing(ctx->stream, &cap));
+  const bool capturing = cap != hipStreamCaptureStatusNone;
+  if (need > ctx->d_gemm_bytes) {
+    if (capturing)
+      return SetError(ctx, EHIP_FAILED_PRECONDITION,
+                      "the call needs a workspace of %zu bytes, and none that large was made before "
+                      "this capture: make the call once outside it",
+                      need);
+    const size_t bytes = std::max(need, ctx->d_gemm_bytes * 3 / 2);
+    EHIP_HIP(ctx, hipStreamSynchronize(ctx->stream));  // queued calls may use the old one
+    if (ctx->d_gemm && ctx->gemm_captured && ctx->n_retired < 64)
+      ctx->retired[ctx->n_retired++] = ctx->d_gemm;
+    else if (ctx->d_gemm)
+      EHIP_HIP(ctx, hipFree(ctx->d_gemm));
+    ctx->d_gemm = nullptr;
+    ctx->d_gemm_bytes = 0;
+    ctx->gemm_captured = false;
+    EHIP_HIP(ctx, hipMalloc(&ctx->d_gemm, bytes));
+    ctx->d_gemm_bytes = bytes;
+  }
+  ctx->gemm_captured = ctx->gemm_captured || capturing;
   return EHIP_OK;
 }
 
@@ -399,6 +433,7 @@ int ehip_destroy(ehip_ctx* ctx) {
   if (ctx->d_desc) (void)hipFree(ctx->d_desc);
   if (ctx->d_part) (void)hipFree(ctx->d_part);
   if (ctx->d_gemm) (void)hipFree(ctx->d_gemm);
+  for (int i = 0; i < ctx->n_retired; ++i) (void)hipFree(ctx->retired[i]);
   if (ctx->d_err) (void)hipFree(ctx->d_err);
   if (ctx->own_stream) (void)hipStreamDestroy(ctx->own_stream);
   delete ctx;
@@ -765,6 +800,29 @@ int ehip_pack_weight_panels(ehip_ctx* ctx, const void* d_w, int32_t weight_dtype
   return EHIP_OK;
 }
 
+namespace {
+
+// The planned linear layer (or gated block) with its workspace: x's bf16
+// planes, then (split k) the partial sums, 256 bytes apart.
+int RunPackedGemm(ehip_ctx* ctx, ehip::GemmParams& p, const float* d_x, int64_t m, int64_t k,
+                  int32_t weight_dtype, int64_t n, float* d_y, bool gated) {
+  ehip::PlanPackedGemm(m, k, n, weight_dtype, ctx->cus, &p, gated);
+  p.x = d_x;
+  p.y = d_y;
+  p.x_vec = (k % 4 == 0 && reinterpret_cast<uintptr_t>(d_x) % 16 == 0) ? 1 : 0;
+  const size_t planes = Align256(ehip::PackedGemmPlaneBytes(p));
+  if (int rc = EnsureGemmWorkspace(ctx, planes + ehip::PackedGemmPartBytes(p))) return rc;
+  p.xp = reinterpret_cast<uint16_t*>(ctx->d_gemm);
+  p.part = p.splits > 1 ? reinterpret_cast<float*>(reinterpret_cast<char*>(ctx->d_gemm) + planes)
+                        : nullptr;
+  EHIP_HIP(ctx, ehip::LaunchPackedGemm(p, weight_dtype, ctx->stream));
+  return EHIP_OK;
+}
+
+bool Aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+}  // namespace
+
 int ehip_packed_gemm(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k, const void* d_wp,
                      int32_t weight_dtype, int64_t n, const float* d_bias, float* d_y) {
   if (int rc = CheckCtx(ctx)) return rc;
@@ -778,36 +836,190 @@ int ehip_packed_gemm(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k, cons
     return SetError(ctx, EHIP_INVALID_ARGUMENT, "gemm: weight_dtype=%d is not F32/BF16/F16",
                     weight_dtype);
   if (!d_x || !d_wp || !d_y) return SetError(ctx, EHIP_INVALID_ARGUMENT, "gemm: null operand");
-  if (reinterpret_cast<uintptr_t>(d_wp) % 16 != 0)
+  if (!Aligned(d_wp, 16))
     return SetError(ctx, EHIP_INVALID_ARGUMENT,
                     "gemm: the packed weight must be 16-byte aligned (ehip_malloc gives 256)");
   ehip::GemmParams p{};
-  ehip::PlanPackedGemm(m, k, n, weight_dtype, ctx->cus, &p);
-  p.x = d_x;
   p.wp = d_wp;
   p.bias = d_bias;
-  p.y = d_y;
-  p.x_vec = (k % 4 == 0 && reinterpret_cast<uintptr_t>(d_x) % 16 == 0) ? 1 : 0;
-  {
-    // x's bf16 planes, then (split k) the partial sums, 256 bytes apart.
-    const size_t planes = (ehip::PackedGemmPlaneBytes(p) + 255) & ~size_t{255};
-    const size_t partial = ehip::PackedGemmPartBytes(p);
-    const size_t need = planes + partial;
-    if (need > ctx->d_gemm_bytes) {
-      const size_t bytes = std::max(need, ctx->d_gemm_bytes * 3 / 2);
-      EHIP_HIP(ctx, hipStreamSynchronize(ctx->stream));  // queued calls may use it
-      if (ctx->d_gemm) EHIP_HIP(ctx, hipFree(ctx->d_gemm));
-      ctx->d_gemm = nullptr;
-      ctx->d_gemm_bytes = 0;
-      EHIP_HIP(ctx, hipMalloc(&ctx->d_gemm, bytes));
-      ctx->d_gemm_bytes = bytes;
-    }
-    p.xp = reinterpret_cast<uint16_t*>(ctx->d_gemm);
-    p.part = p.splits > 1 ? reinterpret_cast<float*>(reinterpret_cast<char*>(ctx->d_gemm) + planes)
-                          : nullptr;
+  return RunPackedGemm(ctx, p, d_x, m, k, weight_dtype, n, d_y, false);
+}
+
+// ------------------------------------------------- feed-forward operators --
+
+namespace {
+
+constexpr int64_t kFfnMost = int64_t{1} << 21;  // rows and widths of the calls below
+
+int CheckSizes(ehip_ctx* ctx, const char* what, int64_t m, int64_t k, int64_t n) {
+  if (m >= 1 && k >= 1 && n >= 1 && m <= kFfnMost && k <= kFfnMost && n <= kFfnMost) return EHIP_OK;
+  return SetError(ctx, EHIP_INVALID_ARGUMENT, "%s: m=%lld k=%lld n=%lld must be in [1, 2^21]", what,
+                  static_cast<long long>(m), static_cast<long long>(k),
+                  static_cast<long long>(n));
+}
+
+int CheckActivation(ehip_ctx* ctx, const char* what, int32_t act) {
+  if (act >= EHIP_ACT_SILU && act <= EHIP_ACT_GELU_TANH) return EHIP_OK;
+  return SetError(ctx, EHIP_INVALID_ARGUMENT, "%s: activation=%d is not SILU/GELU/GELU_TANH", what,
+                  act);
+}
+
+int CheckPanels(ehip_ctx* ctx, const char* what, const void* codes, const void* scales) {
+  if (!codes || !scales) return SetError(ctx, EHIP_INVALID_ARGUMENT, "%s: null panels", what);
+  if (Aligned(codes, 16) && Aligned(scales, 4)) return EHIP_OK;
+  return SetError(ctx, EHIP_INVALID_ARGUMENT,
+                  "%s: codes must be 16-byte and scales 4-byte aligned (ehip_malloc gives 256)",
+                  what);
+}
+
+// The two projections of one call: codes, scales and bias each (the second
+// null for a plain product).
+struct MxWeights {
+  const void* codes[2];
+  const void* scales[2];
+  const float* bias[2];
+};
+
+int RunMxGemm(ehip_ctx* ctx, const void* xc, const void* xs, int64_t m, int64_t k,
+              const MxWeights& w, int64_t n, int32_t act, float* d_y) {
+  ehip::MxGemmParams p{};
+  p.xc = static_cast<const uint8_t*>(xc);
+  p.xs = static_cast<const uint8_t*>(xs);
+  for (int i = 0; i < 2; ++i) {
+    p.wc[i] = static_cast<const uint8_t*>(w.codes[i]);
+    p.ws[i] = static_cast<const uint8_t*>(w.scales[i]);
+    p.bias[i] = w.bias[i];
   }
-  EHIP_HIP(ctx, ehip::LaunchPackedGemm(p, weight_dtype, ctx->stream));
+  p.y = d_y;
+  p.m = m;
+  p.n = n;
+  p.x_panels = ehip::MxPanels(m);
+  p.w_panels = ehip::MxPanels(n);
+  p.tiles = static_cast<int32_t>(ehip::MxTiles(k));
+  p.groups = static_cast<int32_t>(ehip::MxGroups(k));
+  p.y_vec = n % 4 == 0 && Aligned(d_y, 16);
+  p.act = act;
+  EHIP_HIP(ctx, ehip::LaunchMxGemm(p, w.codes[1] != nullptr, ctx->stream));
   return EHIP_OK;
+}
+
+// x quantised into the context's workspace, then the product over it.
+int RunMxLinear(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k, const MxWeights& w,
+                int64_t n, int32_t act, float* d_y) {
+  const size_t codes = static_cast<size_t>(ehip::MxCodeBytes(m, k));
+  if (int rc = EnsureGemmWorkspace(ctx, codes + static_cast<size_t>(ehip::MxScaleBytes(m, k))))
+    return rc;
+  char* xc = reinterpret_cast<char*>(ctx->d_gemm);
+  EHIP_HIP(ctx, ehip::LaunchMxQuantize(d_x, EHIP_WEIGHT_F32, m, k, xc, xc + codes, ctx->stream));
+  return RunMxGemm(ctx, xc, xc + codes, m, k, w, n, act, d_y);
+}
+
+}  // namespace
+
+int ehip_mxfp4_panel_bytes(int64_t rows, int64_t k, int64_t* codes_out, int64_t* scales_out) {
+  if (rows < 1 || k < 1 || rows > kFfnMost || k > kFfnMost) return EHIP_INVALID_ARGUMENT;
+  if (codes_out) *codes_out = ehip::MxCodeBytes(rows, k);
+  if (scales_out) *scales_out = ehip::MxScaleBytes(rows, k);
+  return EHIP_OK;
+}
+
+int ehip_mxfp4_quantize(ehip_ctx* ctx, const void* d_x, int32_t dtype, int64_t rows, int64_t k,
+                        void* d_codes, void* d_scales) {
+  if (int rc = CheckCtx(ctx)) return rc;
+  if (int rc = CheckSizes(ctx, "mxfp4 quantize", rows, k, 1)) return rc;
+  if (!WeightDtypeOk(dtype))
+    return SetError(ctx, EHIP_INVALID_ARGUMENT, "mxfp4 quantize: dtype=%d is not F32/BF16/F16",
+                    dtype);
+  if (!d_x) return SetError(ctx, EHIP_INVALID_ARGUMENT, "mxfp4 quantize: null operand");
+  if (int rc = CheckPanels(ctx, "mxfp4 quantize", d_codes, d_scales)) return rc;
+  EHIP_HIP(ctx, ehip::LaunchMxQuantize(d_x, dtype, rows, k, d_codes, d_scales, ctx->stream));
+  return EHIP_OK;
+}
+
+int ehip_mxfp4_pack(ehip_ctx* ctx, const uint8_t* d_row_codes, const uint8_t* d_row_scales,
+                    int64_t rows, int64_t k, void* d_codes, void* d_scales) {
+  if (int rc = CheckCtx(ctx)) return rc;
+  if (int rc = CheckSizes(ctx, "mxfp4 pack", rows, k, 1)) return rc;
+  if (!d_row_codes || !d_row_scales)
+    return SetError(ctx, EHIP_INVALID_ARGUMENT, "mxfp4 pack: null operand");
+  if (int rc = CheckPanels(ctx, "mxfp4 pack", d_codes, d_scales)) return rc;
+  EHIP_HIP(ctx, ehip::LaunchMxPack(d_row_codes, d_row_scales, rows, k, d_codes, d_scales,
+                                   ctx->stream));
+  return EHIP_OK;
+}
+
+int ehip_mxfp4_dequantize(ehip_ctx* ctx, const void* d_codes, const void* d_scales, int64_t rows,
+                          int64_t k, float* d_y) {
+  if (int rc = CheckCtx(ctx)) return rc;
+  if (int rc = CheckSizes(ctx, "mxfp4 dequantize", rows, k, 1)) return rc;
+  if (!d_y) return SetError(ctx, EHIP_INVALID_ARGUMENT, "mxfp4 dequantize: null operand");
+  if (int rc = CheckPanels(ctx, "mxfp4 dequantize", d_codes, d_scales)) return rc;
+  EHIP_HIP(ctx, ehip::LaunchMxDequantize(d_codes, d_scales, rows, k, d_y, ctx->stream));
+  return EHIP_OK;
+}
+
+int ehip_mxfp4_gemm(ehip_ctx* ctx, const void* d_x_codes, const void* d_x_scales, int64_t m,
+                    int64_t k, const void* d_w_codes, const void* d_w_scales, int64_t n,
+                    const float* d_bias, float* d_y) {
+  if (int rc = CheckCtx(ctx)) return rc;
+  if (int rc = CheckSizes(ctx, "mxfp4 gemm", m, k, n)) return rc;
+  if (int rc = CheckPanels(ctx, "mxfp4 gemm x", d_x_codes, d_x_scales)) return rc;
+  if (int rc = CheckPanels(ctx, "mxfp4 gemm w", d_w_codes, d_w_scales)) return rc;
+  if (!d_y) return SetError(ctx, EHIP_INVALID_ARGUMENT, "mxfp4 gemm: null operand");
+  const MxWeights w{{d_w_codes, nullptr}, {d_w_scales, nullptr}, {d_bias, nullptr}};
+  return RunMxGemm(ctx, d_x_codes, d_x_scales, m, k, w, n, 0, d_y);
+}
+
+int ehip_mxfp4_linear(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k,
+                      const void* d_w_codes, const void* d_w_scales, int64_t n,
+                      const float* d_bias, float* d_y) {
+  if (int rc = CheckCtx(ctx)) return rc;
+  if (int rc = CheckSizes(ctx, "mxfp4 linear", m, k, n)) return rc;
+  if (int rc = CheckPanels(ctx, "mxfp4 linear", d_w_codes, d_w_scales)) return rc;
+  if (!d_x || !d_y) return SetError(ctx, EHIP_INVALID_ARGUMENT, "mxfp4 linear: null operand");
+  const MxWeights w{{d_w_codes, nullptr}, {d_w_scales, nullptr}, {d_bias, nullptr}};
+  return RunMxLinear(ctx, d_x, m, k, w, n, 0, d_y);
+}
+
+int ehip_mxfp4_gated_linear(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k,
+                            const void* d_gate_codes, const void* d_gate_scales,
+                            const void* d_up_codes, const void* d_up_scales, int64_t n,
+                            const float* d_bias_gate, const float* d_bias_up, int32_t activation,
+                            float* d_y) {
+  if (int rc = CheckCtx(ctx)) return rc;
+  if (int rc = CheckSizes(ctx, "mxfp4 gated linear", m, k, n)) return rc;
+  if (int rc = CheckActivation(ctx, "mxfp4 gated linear", activation)) return rc;
+  if (int rc = CheckPanels(ctx, "mxfp4 gated linear gate", d_gate_codes, d_gate_scales)) return rc;
+  if (int rc = CheckPanels(ctx, "mxfp4 gated linear up", d_up_codes, d_up_scales)) return rc;
+  if (!d_x || !d_y) return SetError(ctx, EHIP_INVALID_ARGUMENT, "mxfp4 gated linear: null operand");
+  const MxWeights w{{d_gate_codes, d_up_codes},
+                    {d_gate_scales, d_up_scales},
+                    {d_bias_gate, d_bias_up}};
+  return RunMxLinear(ctx, d_x, m, k, w, n, activation, d_y);
+}
+
+int ehip_packed_gated_gemm(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k,
+                           const void* d_wp_gate, const void* d_wp_up, int32_t weight_dtype,
+                           int64_t n, const float* d_bias_gate, const float* d_bias_up,
+                           int32_t activation, float* d_y) {
+  if (int rc = CheckCtx(ctx)) return rc;
+  if (int rc = CheckSizes(ctx, "gated gemm", m, k, n)) return rc;
+  if (!WeightDtypeOk(weight_dtype))
+    return SetError(ctx, EHIP_INVALID_ARGUMENT, "gated gemm: weight_dtype=%d is not F32/BF16/F16",
+                    weight_dtype);
+  if (int rc = CheckActivation(ctx, "gated gemm", activation)) return rc;
+  if (!d_x || !d_wp_gate || !d_wp_up || !d_y)
+    return SetError(ctx, EHIP_INVALID_ARGUMENT, "gated gemm: null operand");
+  if (!Aligned(d_wp_gate, 16) || !Aligned(d_wp_up, 16))
+    return SetError(ctx, EHIP_INVALID_ARGUMENT,
+                    "gated gemm: the packed weights must be 16-byte aligned (ehip_malloc gives 256)");
+  ehip::GemmParams p{};
+  p.wp = d_wp_gate;
+  p.wp2 = d_wp_up;
+  p.bias = d_bias_gate;
+  p.bias2 = d_bias_up;
+  p.act = activation;
+  return RunPackedGemm(ctx, p, d_x, m, k, weight_dtype, n, d_y, true);
 }
 
 namespace {

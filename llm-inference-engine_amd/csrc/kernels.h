@@ -206,8 +206,8 @@ struct GemmParams {
   const void* wp;       // packed weight
   const float* bias;    // [n] or null
   float* y;             // [m, n]
-  float* part;          // partial sums (splits > 1): [splits, m, n], or with tile_rows > 0
-                        // [split tiles, splits, tile_rows, 256]
+  float* part;          // partial sums (splits > 1): [splits, m, n] (gated: [splits, m, 2, n]),
+                        // or with tile_rows > 0 [split tiles, splits, tile_rows, 256]
   int64_t m, k, n;
   int64_t m_pad, k_pad;  // m, k rounded up to whole 64 x 64 tiles
   int64_t panels;       // ceil(n / 16)
@@ -224,9 +224,16 @@ struct GemmParams {
   int32_t split_steps;
   int32_t items;        // workgroups
   int32_t slots;        // workgroups resident at once
+  // The gated block (projections = 2): y = act(x Wg^T + bias) * (x Wu^T + bias2),
+  // wp the gate's panels and wp2 the up projection's.
+  const void* wp2;
+  const float* bias2;
+  int32_t projections;
+  int32_t act;          // EHIP_ACT_*
 };
 // Tiles and k splits for a call (cus: the device's CU count).
-void PlanPackedGemm(int64_t m, int64_t k, int64_t n, int weight_dtype, int cus, GemmParams* p);
+void PlanPackedGemm(int64_t m, int64_t k, int64_t n, int weight_dtype, int cus, GemmParams* p,
+                    bool gated = false);
 // Workspace bytes of x's planes for the planned call.
 size_t PackedGemmPlaneBytes(const GemmParams& p);
 // Workspace bytes of the planned call's partial sums.
@@ -234,6 +241,37 @@ size_t PackedGemmPartBytes(const GemmParams& p);
 hipError_t LaunchPackedGemm(const GemmParams& p, int weight_dtype, hipStream_t stream);
 hipError_t LaunchPackWeightPanels(const void* w, int weight_dtype, int64_t n, int64_t k, void* wp,
                                   hipStream_t stream);
+
+// MXFP4 (mxfp4.hip; panel layout in mxfp4.h).
+inline int64_t MxPanels(int64_t rows) { return (rows + 15) / 16; }
+inline int64_t MxTiles(int64_t k) { return (k + 127) / 128; }
+inline int64_t MxGroups(int64_t k) { return (MxTiles(k) + 3) / 4; }
+inline int64_t MxCodeBytes(int64_t rows, int64_t k) { return MxPanels(rows) * MxTiles(k) * 1024; }
+inline int64_t MxScaleBytes(int64_t rows, int64_t k) { return MxPanels(rows) * MxGroups(k) * 256; }
+hipError_t LaunchMxQuantize(const void* x, int dtype, int64_t rows, int64_t k, void* codes,
+                            void* scales, hipStream_t stream);
+hipError_t LaunchMxPack(const uint8_t* row_codes, const uint8_t* row_scales, int64_t rows,
+                        int64_t k, void* codes, void* scales, hipStream_t stream);
+hipError_t LaunchMxDequantize(const void* codes, const void* scales, int64_t rows, int64_t k,
+                              float* y, hipStream_t stream);
+
+// y[m, n] = xq wq^T (+ bias[0]), or gated act(xq wq0^T + bias[0]) * (xq wq1^T +
+// bias[1]), over MXFP4 panels.
+struct MxGemmParams {
+  const uint8_t* xc;      // x's codes and scales
+  const uint8_t* xs;
+  const uint8_t* wc[2];   // the projections' codes and scales
+  const uint8_t* ws[2];
+  const float* bias[2];   // [n] or null
+  float* y;               // [m, n]
+  int64_t m, n;
+  int64_t x_panels, w_panels;
+  int32_t tiles;          // 128-k tiles
+  int32_t groups;         // scale groups of 4 tiles
+  int32_t y_vec;          // y rows are 16-byte aligned
+  int32_t act;            // EHIP_ACT_*
+};
+hipError_t LaunchMxGemm(const MxGemmParams& p, bool gated, hipStream_t stream);
 
 hipError_t LaunchFillNormal(void* dst, int64_t n, int dtype, float mean, float stddev,
                             uint64_t seed, hipStream_t stream);

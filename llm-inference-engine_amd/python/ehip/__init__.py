@@ -35,6 +35,10 @@ WEIGHT_F32 = 0
 WEIGHT_BF16 = 1
 WEIGHT_F16 = 2
 
+ACT_SILU = 0
+ACT_GELU = 1
+ACT_GELU_TANH = 2
+
 _i32 = C.c_int32
 _i64 = C.c_int64
 _vp = C.c_void_p
@@ -99,6 +103,16 @@ def lib():
                                                   _i64, _i64, _i64, C.c_float],
             "ehip_pack_weight_panels": [_vp, _vp, _i32, _i64, _i64, _vp],
             "ehip_packed_gemm": [_vp, _vp, _i64, _i64, _vp, _i32, _i64, _vp, _vp],
+            "ehip_packed_gated_gemm": [_vp, _vp, _i64, _i64, _vp, _vp, _i32, _i64, _vp, _vp, _i32,
+                                       _vp],
+            "ehip_mxfp4_panel_bytes": [_i64, _i64, _I64P, _I64P],
+            "ehip_mxfp4_quantize": [_vp, _vp, _i32, _i64, _i64, _vp, _vp],
+            "ehip_mxfp4_pack": [_vp, _vp, _vp, _i64, _i64, _vp, _vp],
+            "ehip_mxfp4_dequantize": [_vp, _vp, _vp, _i64, _i64, _vp],
+            "ehip_mxfp4_gemm": [_vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp],
+            "ehip_mxfp4_linear": [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp],
+            "ehip_mxfp4_gated_linear": [_vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp,
+                                        _i32, _vp],
             "ehip_paged_decode_attention_f32_noalloc": [_vp, _vp, _vp, _vp, _vp, _i64, _i64,
                                                         _i64, _i64, _i64, _i64, _i64, _i64,
                                                         C.c_float, _vp],
@@ -200,6 +214,15 @@ def plan_items(geom: Geometry, step: StepArrays):
     rc = lib().ehip_plan_items(C.byref(geom), C.byref(step.desc), out.ctypes.data, n.value,
                                C.byref(n))
     return rc, out
+
+
+def mxfp4_panel_bytes(rows: int, k: int):
+    """(codes, scales) bytes of a matrix in MXFP4 panels."""
+    c, s = C.c_int64(), C.c_int64()
+    rc = lib().ehip_mxfp4_panel_bytes(rows, k, C.byref(c), C.byref(s))
+    if rc != OK:
+        raise EhipError(rc, f"rows={rows} k={k} must be in [1, 2^21]")
+    return c.value, s.value
 
 
 class DeviceBuffer:
@@ -330,6 +353,48 @@ class Context:
         """Device buffers: y [m, n] = x [m, k] W^T (+ bias) over the packed wp."""
         return lib().ehip_packed_gemm(self.h, x.ptr, m, k, wp.ptr, weight_dtype, n,
                                       bias.ptr if bias is not None else None, y.ptr)
+
+    def packed_gated_gemm(self, x, m, k, wp_gate, wp_up, weight_dtype, n, bias_gate, bias_up,
+                          activation, y) -> int:
+        """Device buffers: y [m, n] = act(x Wg^T + bias_gate) * (x Wu^T + bias_up)
+        over two packed weights."""
+        return lib().ehip_packed_gated_gemm(
+            self.h, x.ptr, m, k, wp_gate.ptr, wp_up.ptr, weight_dtype, n,
+            bias_gate.ptr if bias_gate is not None else None,
+            bias_up.ptr if bias_up is not None else None, activation, y.ptr)
+
+    # --------------------------------------------------------------- MXFP4
+    def mxfp4_quantize(self, x, dtype, rows, k, codes, scales) -> int:
+        """Device buffers: x [rows, k] (WEIGHT_F32/_BF16/_F16) into panels."""
+        return lib().ehip_mxfp4_quantize(self.h, x.ptr, dtype, rows, k, codes.ptr, scales.ptr)
+
+    def mxfp4_pack(self, row_codes, row_scales, rows, k, codes, scales) -> int:
+        """Device buffers: row-major codes and scales into panels."""
+        return lib().ehip_mxfp4_pack(self.h, row_codes.ptr, row_scales.ptr, rows, k, codes.ptr,
+                                     scales.ptr)
+
+    def mxfp4_dequantize(self, codes, scales, rows, k, y) -> int:
+        """Device buffers: panels into their fp32 values y [rows, k]."""
+        return lib().ehip_mxfp4_dequantize(self.h, codes.ptr, scales.ptr, rows, k, y.ptr)
+
+    def mxfp4_gemm(self, x_codes, x_scales, m, k, w_codes, w_scales, n, bias, y) -> int:
+        """Device buffers: y [m, n] = x W^T (+ bias), both operands in panels."""
+        return lib().ehip_mxfp4_gemm(self.h, x_codes.ptr, x_scales.ptr, m, k, w_codes.ptr,
+                                     w_scales.ptr, n, bias.ptr if bias is not None else None,
+                                     y.ptr)
+
+    def mxfp4_linear(self, x, m, k, w_codes, w_scales, n, bias, y) -> int:
+        """Device buffers: y [m, n] = q(x) W^T (+ bias), x [m, k] fp32."""
+        return lib().ehip_mxfp4_linear(self.h, x.ptr, m, k, w_codes.ptr, w_scales.ptr, n,
+                                       bias.ptr if bias is not None else None, y.ptr)
+
+    def mxfp4_gated_linear(self, x, m, k, gate_codes, gate_scales, up_codes, up_scales, n,
+                           bias_gate, bias_up, activation, y) -> int:
+        """Device buffers: y [m, n] = act(q(x) Wg^T + bias_gate) * (q(x) Wu^T + bias_up)."""
+        return lib().ehip_mxfp4_gated_linear(
+            self.h, x.ptr, m, k, gate_codes.ptr, gate_scales.ptr, up_codes.ptr, up_scales.ptr, n,
+            bias_gate.ptr if bias_gate is not None else None,
+            bias_up.ptr if bias_up is not None else None, activation, y.ptr)
 
     def paged_decode_batched(self, q, k_slab, v_slab, tables, lengths, heads, kv_heads, d, bs,
                              block_stride, slab_blocks, scale, out, bf16=False) -> int:
