@@ -270,6 +270,7 @@ struct MxGemmParams {
   int32_t groups;         // scale groups of 4 tiles
   int32_t y_vec;          // y rows are 16-byte aligned
   int32_t act;            // EHIP_ACT_*
+  int32_t row_tiles, col_tiles;  // the staged kernel's (set at its launch)
 };
 hipError_t LaunchMxGemm(const MxGemmParams& p, bool gated, hipStream_t stream);
 

@@ -192,19 +192,23 @@ __device__ __forceinline__ f32x4_t MxMfma(const i32x4_t& w, uint32_t ws, const i
                                                           static_cast<int>(xs));
 }
 
+// ACT of a plain product; gated ones name their activation, so that a kernel
+// holds one activation's code (erfc alone is a hundred instructions a value).
+constexpr int kPlain = -1;
+
 // One fragment's results: row n16 of an x panel, columns 4 q .. + 3 of a weight
-// panel; `up` the other projection's sums where GATED.
-template <bool GATED>
+// panel; `up` the other projection's sums of a gated call.
+template <int ACT>
 __device__ __forceinline__ void MxStore(const MxGemmParams& p, int64_t row, int64_t col,
                                         f32x4_t g, f32x4_t up) {
-  if (row >= p.m) return;
+  if (row >= p.m || col >= p.n) return;
   float out[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const bool in = col + i < p.n;
     float v = g[i] + (in && p.bias[0] ? p.bias[0][col + i] : 0.f);
-    if constexpr (GATED)
-      v = Activate(p.act, v) * (up[i] + (in && p.bias[1] ? p.bias[1][col + i] : 0.f));
+    if constexpr (ACT != kPlain)
+      v = Activate<ACT>(v) * (up[i] + (in && p.bias[1] ? p.bias[1][col + i] : 0.f));
     out[i] = v;
   }
   float* y = p.y + row * p.n + col;
@@ -220,9 +224,9 @@ __device__ __forceinline__ void MxStore(const MxGemmParams& p, int64_t row, int6
 // Few rows: a workgroup per (MP x panels, NP weight panels), its KW wavefronts
 // taking the scale groups in turn with their operands straight from memory into
 // registers, then one sum over the wavefronts through LDS, in their order.
-template <int MP, int NP, bool GATED, int KW>
+template <int MP, int NP, int ACT, int KW>
 __global__ __launch_bounds__(64 * KW) void MxDirect(MxGemmParams p) {
-  constexpr int PR = GATED ? 2 : 1;
+  constexpr int PR = ACT != kPlain ? 2 : 1;
   __shared__ f32x4_t red[KW][MP * NP * PR][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -290,20 +294,204 @@ __global__ __launch_bounds__(64 * KW) void MxDirect(MxGemmParams p) {
     }
     const int64_t row = (xp0 + f / NP) * kMxRows + (lane & 15);
     const int64_t panel = wp0 + f % NP;
-    if (panel < p.w_panels) MxStore<GATED>(p, row, panel * kMxRows + 4 * (lane >> 4), s[0], s[PR - 1]);
+    if (panel < p.w_panels) MxStore<ACT>(p, row, panel * kMxRows + 4 * (lane >> 4), s[0], s[PR - 1]);
   }
 }
 
-template <bool GATED>
+// Many rows: a workgroup of WR x WC wavefronts per tile of WR XP x panels by WC WP
+// weight panels (gated: their even slots the gate's, the odd ones the up
+// projection's). k tiles go from memory straight into LDS (buffer_load ... lds, a
+// panel's 1 KiB an instruction, four a wavefront), into four buffers, three
+// tiles ahead; an operand is one conflict-free 16-byte read. A wavefront's
+// scales, one dword a panel and group, come through registers a group ahead.
+template <int WR, int WC, int XP, int WP, int ACT, int OCC>
+__global__ __launch_bounds__(64 * WR * WC) __attribute__((amdgpu_waves_per_eu(OCC)))
+void MxStaged(MxGemmParams p) {
+  constexpr bool GATED = ACT != kPlain;
+  constexpr int XT = WR * XP, WT = WC * WP;  // panels of the tile
+  static_assert(XT + WT == 4 * WR * WC && XT % 4 == 0, "four panels a wavefront");
+  static_assert(!GATED || WP % 2 == 0, "pairs of slots");
+  __shared__ __align__(16) unsigned char b0[(XT + WT) * kMxTileBytes];
+  __shared__ __align__(16) unsigned char b1[(XT + WT) * kMxTileBytes];
+  __shared__ __align__(16) unsigned char b2[(XT + WT) * kMxTileBytes];
+  __shared__ __align__(16) unsigned char b3[(XT + WT) * kMxTileBytes];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int wr = wave / WC, wc = wave % WC;
+
+  // Tiles in bands of 4 rows of tiles, columns outer within a band; an XCD (b
+  // mod 8) takes consecutive ones, which share their panels in its L2.
+  const uint32_t tiles_all = static_cast<uint32_t>(p.row_tiles) * p.col_tiles;
+  const uint32_t per = (tiles_all + 7) / 8;
+  const uint32_t tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (tile >= tiles_all) return;
+  const uint32_t band = tile / (4u * p.col_tiles);
+  const uint32_t in_band = tile - band * 4u * p.col_tiles;
+  const uint32_t h = min(4u, static_cast<uint32_t>(p.row_tiles) - 4u * band);
+  const int ct = __builtin_amdgcn_readfirstlane(in_band / h);
+  const int rt = __builtin_amdgcn_readfirstlane(4 * band + in_band % h);
+  const int64_t xp0 = int64_t{rt} * XT;
+  const int64_t wp0 = int64_t{ct} * (GATED ? WT / 2 : WT);
+  const int last_x = static_cast<int>(min(int64_t{XT}, p.x_panels - xp0)) - 1;
+  const int last_w = static_cast<int>(min(int64_t{WT}, p.w_panels - wp0)) - 1;
+
+  // The wavefront's four panels of a stage: all of x, or all weight slots.
+  // Panels past the last read the last one: their results are not stored.
+  const int slot = 4 * wave;
+  const bool is_x = slot < XT;
+  const int64_t row_bytes = int64_t{p.tiles} * kMxTileBytes;
+  const uint8_t* const even = is_x ? p.xc + xp0 * row_bytes : p.wc[0] + wp0 * row_bytes;
+  const uint8_t* const odd = is_x || !GATED ? even : p.wc[1] + wp0 * row_bytes;
+  const __amdgpu_buffer_rsrc_t re = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(even), 0, 0xFFFFFFFFu, 0x00020000);
+  const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(odd), 0, 0xFFFFFFFFu, 0x00020000);
+  uint32_t src[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int local = is_x ? min(slot + i, last_x)
+                           : min(GATED ? (slot - XT + i) / 2 : slot - XT + i, last_w);
+    src[i] = static_cast<uint32_t>(local) * static_cast<uint32_t>(row_bytes);
+  }
+  auto stage = [&](unsigned char* buf, int t) __attribute__((always_inline)) {
+    const uint32_t at = static_cast<uint32_t>(min(t, p.tiles - 1)) * kMxTileBytes;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          i & 1 ? ro : re,
+          (__attribute__((address_space(3))) void*)(buf + (slot + i) * kMxTileBytes), 16,
+          lane * 16, src[i] + at, 0, 0);
+  };
+
+  // Scales of the wavefront's own panels.
+  const int64_t row_scales = int64_t{p.groups} * kMxScaleBytes;
+  const __amdgpu_buffer_rsrc_t rxs = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(p.xs + xp0 * row_scales), 0, 0xFFFFFFFFu, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rg = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(p.ws[0] + wp0 * row_scales), 0, 0xFFFFFFFFu, 0x00020000);
+  const __amdgpu_buffer_rsrc_t ru =
+      GATED ? __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.ws[1] + wp0 * row_scales), 0,
+                                                0xFFFFFFFFu, 0x00020000)
+            : rg;
+  auto load_scales = [&](int g, uint32_t (&sx)[XP], uint32_t (&sw)[WP])
+                         __attribute__((always_inline)) {
+    const uint32_t at = static_cast<uint32_t>(min(g, p.groups - 1)) * kMxScaleBytes;
+    const uint32_t rs = static_cast<uint32_t>(row_scales);
+#pragma unroll
+    for (int a = 0; a < XP; ++a)
+      sx[a] = __builtin_amdgcn_raw_buffer_load_b32(
+          rxs, lane * 4, static_cast<uint32_t>(min(wr * XP + a, last_x)) * rs + at, 0);
+#pragma unroll
+    for (int b = 0; b < WP; ++b) {
+      const int local = min(GATED ? (wc * WP + b) / 2 : wc * WP + b, last_w);
+      sw[b] = __builtin_amdgcn_raw_buffer_load_b32(GATED && (b & 1) ? ru : rg, lane * 4,
+                                                   static_cast<uint32_t>(local) * rs + at, 0);
+    }
+  };
+
+  f32x4_t acc[XP][WP];
+#pragma unroll
+  for (int a = 0; a < XP; ++a)
+#pragma unroll
+    for (int b = 0; b < WP; ++b) acc[a][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  uint32_t sx[XP], sw[WP], nx[XP], nw[WP];
+
+#define EHIP_MX_FENCE() asm volatile("" ::: "memory")
+  load_scales(0, sx, sw);
+  EHIP_MX_FENCE();
+  stage(b0, 0);
+  EHIP_MX_FENCE();
+  stage(b1, 1);
+  EHIP_MX_FENCE();
+  stage(b2, 2);
+  EHIP_MX_FENCE();
+  auto compute = [&](auto j, const unsigned char* buf) __attribute__((always_inline)) {
+    constexpr int J = decltype(j)::value;
+    i32x4_t w[WP];
+#pragma unroll
+    for (int b = 0; b < WP; ++b)
+      w[b] = *reinterpret_cast<const i32x4_t*>(buf + (XT + wc * WP + b) * kMxTileBytes + lane * 16);
+#pragma unroll
+    for (int a = 0; a < XP; ++a) {
+      const i32x4_t x =
+          *reinterpret_cast<const i32x4_t*>(buf + (wr * XP + a) * kMxTileBytes + lane * 16);
+#pragma unroll
+      for (int b = 0; b < WP; ++b) acc[a][b] = MxMfma<J>(w[b], sw[b], x, sx[a], acc[a][b]);
+    }
+  };
+  // Step t waits for its own tile's loads and meets the other wavefronts', then
+  // loads tile t + 3 into the buffer that step t - 1 has read. The loads stay
+  // unconditional (past the end: the last tile again), so that the counts
+  // hold: behind a tile's loads are two more tiles' (8), and at J = 1 and 2 the
+  // next group's XP + WP scales, which are loaded at J = 0.
+#define EHIP_MX_STEP(J, BUF, NEXT, PENDING)                                                  \
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PENDING) : "memory");      \
+  if ((J) == 0) {                                                                            \
+    load_scales(g + 1, nx, nw);                                                              \
+    EHIP_MX_FENCE();                                                                         \
+  }                                                                                          \
+  stage(NEXT, 4 * g + (J) + 3);                                                              \
+  EHIP_MX_FENCE();                                                                           \
+  compute(std::integral_constant<int, (J)>{}, BUF);                                          \
+  if (4 * g + (J) + 1 >= p.tiles) break
+  for (int g = 0;; ++g) {
+    EHIP_MX_STEP(0, b0, b3, 8);
+    EHIP_MX_STEP(1, b1, b0, 8 + XP + WP);
+    EHIP_MX_STEP(2, b2, b1, 8 + XP + WP);
+    EHIP_MX_STEP(3, b3, b2, 8);
+#pragma unroll
+    for (int a = 0; a < XP; ++a) sx[a] = nx[a];
+#pragma unroll
+    for (int b = 0; b < WP; ++b) sw[b] = nw[b];
+  }
+  // Loads past the end may still be in flight: they write this workgroup's
+  // LDS, so they land before it ends.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#undef EHIP_MX_STEP
+#undef EHIP_MX_FENCE
+
+#pragma unroll
+  for (int a = 0; a < XP; ++a) {
+    const int64_t row = (xp0 + wr * XP + a) * kMxRows + (lane & 15);
+#pragma unroll
+    for (int b = 0; b < WP; b += GATED ? 2 : 1) {
+      const int64_t panel = wp0 + (GATED ? (wc * WP + b) / 2 : wc * WP + b);
+      MxStore<ACT>(p, row, panel * kMxRows + 4 * (lane >> 4), acc[a][b],
+                     acc[a][GATED ? b + 1 : b]);
+    }
+  }
+}
+
+template <int WR, int WC, int XP, int WP, int ACT, int OCC>
+hipError_t LaunchStaged(MxGemmParams p, hipStream_t stream) {
+  constexpr int64_t XT = WR * XP, WT = ACT != kPlain ? WC * WP / 2 : WC * WP;
+  const int64_t rt = (p.x_panels + XT - 1) / XT, ct = (p.w_panels + WT - 1) / WT;
+  if (rt * ct > (int64_t{1} << 30)) return hipErrorInvalidValue;
+  p.row_tiles = static_cast<int32_t>(rt);
+  p.col_tiles = static_cast<int32_t>(ct);
+  const uint32_t grid = static_cast<uint32_t>((rt * ct + 7) / 8 * 8);
+  hipLaunchKernelGGL((MxStaged<WR, WC, XP, WP, ACT, OCC>), dim3(grid), dim3(64 * WR * WC), 0,
+                     stream, p);
+  return hipGetLastError();
+}
+
+template <int ACT>
 hipError_t LaunchDirect(const MxGemmParams& p, hipStream_t stream) {
   const int64_t n = p.w_panels * ((p.x_panels + 3) / 4);
   if (n > INT32_MAX) return hipErrorInvalidValue;
   const dim3 grid(static_cast<uint32_t>(n));
   if (p.x_panels == 1)
-    hipLaunchKernelGGL((MxDirect<1, 1, GATED, 8>), grid, dim3(512), 0, stream, p);
+    hipLaunchKernelGGL((MxDirect<1, 1, ACT, 8>), grid, dim3(512), 0, stream, p);
   else
-    hipLaunchKernelGGL((MxDirect<4, 1, GATED, 8>), grid, dim3(512), 0, stream, p);
+    hipLaunchKernelGGL((MxDirect<4, 1, ACT, 8>), grid, dim3(512), 0, stream, p);
   return hipGetLastError();
+}
+
+template <int ACT>
+hipError_t LaunchProduct(const MxGemmParams& p, hipStream_t stream) {
+  if (p.m > 256) return LaunchStaged<2, 4, 8, 4, ACT, 2>(p, stream);
+  if (p.m > 64) return LaunchStaged<2, 2, 4, 4, ACT, 2>(p, stream);
+  return LaunchDirect<ACT>(p, stream);
 }
 
 // Workgroups of the panel conversions, 0 where a launch cannot hold them.
@@ -351,7 +539,12 @@ hipError_t LaunchMxDequantize(const void* codes, const void* scales, int64_t row
 }
 
 hipError_t LaunchMxGemm(const MxGemmParams& p, bool gated, hipStream_t stream) {
-  return gated ? LaunchDirect<true>(p, stream) : LaunchDirect<false>(p, stream);
+  if (!gated) return LaunchProduct<kPlain>(p, stream);
+  switch (p.act) {
+    case EHIP_ACT_SILU: return LaunchProduct<EHIP_ACT_SILU>(p, stream);
+    case EHIP_ACT_GELU: return LaunchProduct<EHIP_ACT_GELU>(p, stream);
+    default: return LaunchProduct<EHIP_ACT_GELU_TANH>(p, stream);
+  }
 }
 
 }  // namespace ehip
