@@ -880,9 +880,11 @@ struct MxWeights {
   const float* bias[2];
 };
 
-int RunMxGemm(ehip_ctx* ctx, const void* xc, const void* xs, int64_t m, int64_t k,
+// x as fp32 rows or (x null) as panels.
+int RunMxGemm(ehip_ctx* ctx, const float* x, const void* xc, const void* xs, int64_t m, int64_t k,
               const MxWeights& w, int64_t n, int32_t act, float* d_y) {
   ehip::MxGemmParams p{};
+  p.x = x;
   p.xc = static_cast<const uint8_t*>(xc);
   p.xs = static_cast<const uint8_t*>(xs);
   for (int i = 0; i < 2; ++i) {
@@ -892,26 +894,31 @@ int RunMxGemm(ehip_ctx* ctx, const void* xc, const void* xs, int64_t m, int64_t 
   }
   p.y = d_y;
   p.m = m;
+  p.k = k;
   p.n = n;
   p.x_panels = ehip::MxPanels(m);
   p.w_panels = ehip::MxPanels(n);
   p.tiles = static_cast<int32_t>(ehip::MxTiles(k));
   p.groups = static_cast<int32_t>(ehip::MxGroups(k));
+  p.x_vec = k % 4 == 0 && Aligned(x, 16);
   p.y_vec = n % 4 == 0 && Aligned(d_y, 16);
   p.act = act;
   EHIP_HIP(ctx, ehip::LaunchMxGemm(p, w.codes[1] != nullptr, ctx->stream));
   return EHIP_OK;
 }
 
-// x quantised into the context's workspace, then the product over it.
+// x quantised into the context's workspace, then the product over it; few rows
+// in the product's own kernel.
 int RunMxLinear(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k, const MxWeights& w,
                 int64_t n, int32_t act, float* d_y) {
+  if (ehip::MxFusesQuantization(m))
+    return RunMxGemm(ctx, d_x, nullptr, nullptr, m, k, w, n, act, d_y);
   const size_t codes = static_cast<size_t>(ehip::MxCodeBytes(m, k));
   if (int rc = EnsureGemmWorkspace(ctx, codes + static_cast<size_t>(ehip::MxScaleBytes(m, k))))
     return rc;
   char* xc = reinterpret_cast<char*>(ctx->d_gemm);
   EHIP_HIP(ctx, ehip::LaunchMxQuantize(d_x, EHIP_WEIGHT_F32, m, k, xc, xc + codes, ctx->stream));
-  return RunMxGemm(ctx, xc, xc + codes, m, k, w, n, act, d_y);
+  return RunMxGemm(ctx, nullptr, xc, xc + codes, m, k, w, n, act, d_y);
 }
 
 }  // namespace
@@ -967,7 +974,7 @@ int ehip_mxfp4_gemm(ehip_ctx* ctx, const void* d_x_codes, const void* d_x_scales
   if (int rc = CheckPanels(ctx, "mxfp4 gemm w", d_w_codes, d_w_scales)) return rc;
   if (!d_y) return SetError(ctx, EHIP_INVALID_ARGUMENT, "mxfp4 gemm: null operand");
   const MxWeights w{{d_w_codes, nullptr}, {d_w_scales, nullptr}, {d_bias, nullptr}};
-  return RunMxGemm(ctx, d_x_codes, d_x_scales, m, k, w, n, 0, d_y);
+  return RunMxGemm(ctx, nullptr, d_x_codes, d_x_scales, m, k, w, n, 0, d_y);
 }
 
 int ehip_mxfp4_linear(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k,

@@ -258,20 +258,24 @@ hipError_t LaunchMxDequantize(const void* codes, const void* scales, int64_t row
 // y[m, n] = xq wq^T (+ bias[0]), or gated act(xq wq0^T + bias[0]) * (xq wq1^T +
 // bias[1]), over MXFP4 panels.
 struct MxGemmParams {
+  const float* x;         // x in fp32 rows [m, k], quantised by the kernel; null: panels
   const uint8_t* xc;      // x's codes and scales
   const uint8_t* xs;
   const uint8_t* wc[2];   // the projections' codes and scales
   const uint8_t* ws[2];
   const float* bias[2];   // [n] or null
   float* y;               // [m, n]
-  int64_t m, n;
+  int64_t m, k, n;
   int64_t x_panels, w_panels;
   int32_t tiles;          // 128-k tiles
   int32_t groups;         // scale groups of 4 tiles
+  int32_t x_vec;          // x rows are 16-byte aligned
   int32_t y_vec;          // y rows are 16-byte aligned
   int32_t act;            // EHIP_ACT_*
   int32_t row_tiles, col_tiles;  // the staged kernel's (set at its launch)
 };
+// Whether a product of m fp32 rows quantises them itself.
+bool MxFusesQuantization(int64_t m);
 hipError_t LaunchMxGemm(const MxGemmParams& p, bool gated, hipStream_t stream);
 
 hipError_t LaunchFillNormal(void* dst, int64_t n, int dtype, float mean, float stddev,

@@ -38,20 +38,15 @@ __device__ __forceinline__ uint32_t MxScaleByte(uint32_t amax) {
 }
 
 // Eight values as E2M1 codes of v / 2^(byte - 127), nearest even and at most 6
-// in magnitude: ldexp is exact here (what it could round is below half the
-// smallest code), so the conversion rounds once.
+// in magnitude. The conversion takes the scale's exponent from a float's.
 __device__ __forceinline__ uint32_t MxCodes(const float (&v)[8], uint32_t byte) {
   if (byte == 255u) return 0u;
-  const int up = 127 - static_cast<int>(byte);
+  const float scale = __uint_as_float(byte << 23);
   uint32_t r = 0;
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, __builtin_amdgcn_ldexpf(v[0], up),
-                                               __builtin_amdgcn_ldexpf(v[1], up), 1.f, 0);
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, __builtin_amdgcn_ldexpf(v[2], up),
-                                               __builtin_amdgcn_ldexpf(v[3], up), 1.f, 1);
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, __builtin_amdgcn_ldexpf(v[4], up),
-                                               __builtin_amdgcn_ldexpf(v[5], up), 1.f, 2);
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, __builtin_amdgcn_ldexpf(v[6], up),
-                                               __builtin_amdgcn_ldexpf(v[7], up), 1.f, 3);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[0], v[1], scale, 0);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], scale, 1);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4], v[5], scale, 2);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], scale, 3);
   return r;
 }
 

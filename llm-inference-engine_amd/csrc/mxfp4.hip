@@ -196,53 +196,79 @@ __device__ __forceinline__ f32x4_t MxMfma(const i32x4_t& w, uint32_t ws, const i
 // holds one activation's code (erfc alone is a hundred instructions a value).
 constexpr int kPlain = -1;
 
-// One fragment's results: row n16 of an x panel, columns 4 q .. + 3 of a weight
-// panel; `up` the other projection's sums of a gated call.
+// Biases, then the activation and the product, of four columns from `col`:
+// `up` the other projection's sums of a gated call.
 template <int ACT>
-__device__ __forceinline__ void MxStore(const MxGemmParams& p, int64_t row, int64_t col,
-                                        f32x4_t g, f32x4_t up) {
-  if (row >= p.m || col >= p.n) return;
-  float out[4];
+__device__ __forceinline__ f32x4_t MxFinish(const MxGemmParams& p, int64_t col, f32x4_t g,
+                                            f32x4_t up) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const bool in = col + i < p.n;
     float v = g[i] + (in && p.bias[0] ? p.bias[0][col + i] : 0.f);
     if constexpr (ACT != kPlain)
       v = Activate<ACT>(v) * (up[i] + (in && p.bias[1] ? p.bias[1][col + i] : 0.f));
-    out[i] = v;
+    g[i] = v;
   }
+  return g;
+}
+
+// Four columns of a row of y, as far as they lie in it.
+__device__ __forceinline__ void MxStore(const MxGemmParams& p, int64_t row, int64_t col,
+                                        const f32x4_t& v) {
+  if (row >= p.m || col >= p.n) return;
   float* y = p.y + row * p.n + col;
-  if (p.y_vec && col + 4 <= p.n) {
-    *reinterpret_cast<float4*>(y) = make_float4(out[0], out[1], out[2], out[3]);
+  if (p.y_vec) {  // n % 4 == 0
+    __builtin_nontemporal_store(v, reinterpret_cast<f32x4_t*>(y));
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (col + i < p.n) y[i] = out[i];
+      if (col + i < p.n) y[i] = v[i];
   }
 }
 
-// Few rows: a workgroup per (MP x panels, NP weight panels), its KW wavefronts
-// taking the scale groups in turn with their operands straight from memory into
-// registers, then one sum over the wavefronts through LDS, in their order.
-template <int MP, int NP, int ACT, int KW>
+// 32 values of one block as codes and the scale byte.
+__device__ __forceinline__ i32x4_t MxBlock(const f32x4_t (&v)[8], uint32_t* byte) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = __builtin_elementwise_maximum(top, fabsf(v[i][e]));
+  *byte = MxScaleByte(__float_as_uint(top) & 0x7FFFFFFFu);
+  i32x4_t codes;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float w[8] = {v[2 * i][0],     v[2 * i][1],     v[2 * i][2],     v[2 * i][3],
+                        v[2 * i + 1][0], v[2 * i + 1][1], v[2 * i + 1][2], v[2 * i + 1][3]};
+    codes[i] = static_cast<int>(MxCodes(w, *byte));
+  }
+  return codes;
+}
+
+// Few rows: a workgroup per (MP x panels, one weight panel a projection), its KW
+// wavefronts taking the scale groups in turn with their operands straight from
+// memory into registers, a group ahead, then one sum over the wavefronts through
+// LDS, in their order. FUSED (MP = 1): x is fp32 rows, and a lane quantises its
+// own block.
+template <int MP, int ACT, int KW, bool FUSED>
 __global__ __launch_bounds__(64 * KW) void MxDirect(MxGemmParams p) {
+  static_assert(!FUSED || MP == 1, "fused quantisation of one panel");
   constexpr int PR = ACT != kPlain ? 2 : 1;
-  __shared__ f32x4_t red[KW][MP * NP * PR][64];
+  __shared__ f32x4_t red[KW][MP * PR][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  const uint32_t w_groups = static_cast<uint32_t>((p.w_panels + NP - 1) / NP);
-  const uint32_t xb = blockIdx.x / w_groups;
-  const int64_t wp0 = int64_t{blockIdx.x - xb * w_groups} * NP, xp0 = int64_t{xb} * MP;
-  f32x4_t acc[MP][NP * PR];
+  const uint32_t xb = blockIdx.x / static_cast<uint32_t>(p.w_panels);
+  const int64_t wp = blockIdx.x - xb * static_cast<uint32_t>(p.w_panels);
+  const int64_t xp0 = int64_t{xb} * MP;
+  f32x4_t acc[MP][PR];
 #pragma unroll
   for (int a = 0; a < MP; ++a)
 #pragma unroll
-    for (int b = 0; b < NP * PR; ++b) acc[a][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  // Panels past the last read the last one: their results are not stored.
+    for (int b = 0; b < PR; ++b) acc[a][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  // x panels past the last read the last one: their results are not stored.
   const i32x4_t* xc[MP];
   const uint32_t* xs[MP];
-  const i32x4_t* wc[NP * PR];
-  const uint32_t* ws[NP * PR];
+  const i32x4_t* wc[PR];
+  const uint32_t* ws[PR];
 #pragma unroll
   for (int a = 0; a < MP; ++a) {
     const int64_t panel = min(xp0 + a, p.x_panels - 1);
@@ -250,30 +276,81 @@ __global__ __launch_bounds__(64 * KW) void MxDirect(MxGemmParams p) {
     xs[a] = reinterpret_cast<const uint32_t*>(p.xs) + panel * p.groups * 64 + lane;
   }
 #pragma unroll
-  for (int b = 0; b < NP * PR; ++b) {
-    const int64_t panel = min(wp0 + b / PR, p.w_panels - 1);
-    wc[b] = reinterpret_cast<const i32x4_t*>(p.wc[b % PR]) + panel * p.tiles * 64 + lane;
-    ws[b] = reinterpret_cast<const uint32_t*>(p.ws[b % PR]) + panel * p.groups * 64 + lane;
+  for (int b = 0; b < PR; ++b) {
+    wc[b] = reinterpret_cast<const i32x4_t*>(p.wc[b]) + wp * p.tiles * 64 + lane;
+    ws[b] = reinterpret_cast<const uint32_t*>(p.ws[b]) + wp * p.groups * 64 + lane;
+  }
+  const int row = lane & 15, block = lane >> 4;
+  const bool live = row < p.m;
+  const float* const xf = FUSED ? p.x + int64_t{live ? row : 0} * p.k : nullptr;
+
+  i32x4_t x[kMxGroup][MP], w[kMxGroup][PR];
+  uint32_t sx[MP], sw[PR];
+  auto load_scales = [&](int t) __attribute__((always_inline)) {
+    if constexpr (!FUSED) {
+#pragma unroll
+      for (int a = 0; a < MP; ++a) sx[a] = xs[a][int64_t{t} * 64];
+    }
+#pragma unroll
+    for (int b = 0; b < PR; ++b) sw[b] = ws[b][int64_t{t} * 64];
+  };
+  auto load = [&](int t, int j) __attribute__((always_inline)) {
+    const int64_t tile = min(t * kMxGroup + j, p.tiles - 1);
+    if constexpr (!FUSED) {
+#pragma unroll
+      for (int a = 0; a < MP; ++a) x[j][a] = xc[a][tile * 64];
+    }
+#pragma unroll
+    for (int b = 0; b < PR; ++b) w[j][b] = wc[b][tile * 64];
+  };
+  if (wave < p.groups) {
+    load_scales(wave);
+#pragma unroll
+    for (int j = 0; j < kMxGroup; ++j) load(wave, j);
   }
   for (int t = wave; t < p.groups; t += KW) {
-    uint32_t sx[MP], sw[NP * PR];
+    uint32_t cx[MP], cw[PR];
 #pragma unroll
-    for (int a = 0; a < MP; ++a) sx[a] = xs[a][int64_t{t} * 64];
+    for (int b = 0; b < PR; ++b) cw[b] = sw[b];
+    if constexpr (FUSED) {
+      // The codes of the group's blocks; byte j of the scales is tile j's.
+      cx[0] = 0;
 #pragma unroll
-    for (int b = 0; b < NP * PR; ++b) sw[b] = ws[b][int64_t{t} * 64];
+      for (int j = 0; j < kMxGroup; ++j) {
+        const int64_t k0 = (int64_t{t} * kMxGroup + j) * kMxTile + block * kMxBlock;
+        f32x4_t v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        if (live && p.x_vec && k0 + kMxBlock <= p.k) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const f32x4_t*>(xf + k0 + 4 * i);
+        } else if (live) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (k0 + 4 * i + e < p.k) v[i][e] = xf[k0 + 4 * i + e];
+        }
+        uint32_t byte;
+        x[j][0] = MxBlock(v, &byte);
+        cx[0] |= byte << (8 * j);
+      }
+    } else {
+#pragma unroll
+      for (int a = 0; a < MP; ++a) cx[a] = sx[a];
+    }
+    const bool more = t + KW < p.groups;
+    if (more) load_scales(t + KW);
     auto step = [&](auto j) __attribute__((always_inline)) {
       constexpr int J = decltype(j)::value;
-      const int64_t tile = int64_t{t} * kMxGroup + J;
-      if (tile >= p.tiles) return;
-      i32x4_t x[MP];
+      if (t * kMxGroup + J < p.tiles) {
 #pragma unroll
-      for (int a = 0; a < MP; ++a) x[a] = xc[a][tile * 64];
+        for (int b = 0; b < PR; ++b)
 #pragma unroll
-      for (int b = 0; b < NP * PR; ++b) {
-        const i32x4_t w = wc[b][tile * 64];
-#pragma unroll
-        for (int a = 0; a < MP; ++a) acc[a][b] = MxMfma<J>(w, sw[b], x[a], sx[a], acc[a][b]);
+          for (int a = 0; a < MP; ++a)
+            acc[a][b] = MxMfma<J>(w[J][b], cw[b], x[J][a], cx[a], acc[a][b]);
       }
+      if (more) load(t + KW, J);
     };
     step(std::integral_constant<int, 0>{});
     step(std::integral_constant<int, 1>{});
@@ -283,38 +360,54 @@ __global__ __launch_bounds__(64 * KW) void MxDirect(MxGemmParams p) {
 #pragma unroll
   for (int a = 0; a < MP; ++a)
 #pragma unroll
-    for (int b = 0; b < NP * PR; ++b) red[wave][a * NP * PR + b][lane] = acc[a][b];
+    for (int b = 0; b < PR; ++b) red[wave][a * PR + b][lane] = acc[a][b];
   __syncthreads();
-  for (int f = wave; f < MP * NP; f += KW) {
+  for (int f = wave; f < MP; f += KW) {
     f32x4_t s[PR];
 #pragma unroll
     for (int h = 0; h < PR; ++h) {
       s[h] = red[0][f * PR + h][lane];
-      for (int w = 1; w < KW; ++w) s[h] += red[w][f * PR + h][lane];
+#pragma unroll 4
+      for (int i = 1; i < KW; ++i) s[h] += red[i][f * PR + h][lane];
     }
-    const int64_t row = (xp0 + f / NP) * kMxRows + (lane & 15);
-    const int64_t panel = wp0 + f % NP;
-    if (panel < p.w_panels) MxStore<ACT>(p, row, panel * kMxRows + 4 * (lane >> 4), s[0], s[PR - 1]);
+    const int64_t col = wp * kMxRows + 4 * block;
+    MxStore(p, (xp0 + f) * kMxRows + row, col, MxFinish<ACT>(p, col, s[0], s[PR - 1]));
   }
+}
+
+template <int I>
+__device__ __forceinline__ unsigned char* Buffer(unsigned char* b0, unsigned char* b1,
+                                                 unsigned char* b2, unsigned char* b3) {
+  return I == 0 ? b0 : I == 1 ? b1 : I == 2 ? b2 : b3;
+}
+
+// Waits until no more than N vector-memory operations and no LDS one of the
+// wavefront are outstanding, then for the other wavefronts.
+template <int N>
+__device__ __forceinline__ void WaitAndMeet() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
 // Many rows: a workgroup of WR x WC wavefronts per tile of WR XP x panels by WC WP
 // weight panels (gated: their even slots the gate's, the odd ones the up
 // projection's). k tiles go from memory straight into LDS (buffer_load ... lds, a
-// panel's 1 KiB an instruction, four a wavefront), into four buffers, three
-// tiles ahead; an operand is one conflict-free 16-byte read. A wavefront's
-// scales, one dword a panel and group, come through registers a group ahead.
-template <int WR, int WC, int XP, int WP, int ACT, int OCC>
+// panel's 1 KiB an instruction), into NS buffers, NS - 1 tiles ahead; an operand
+// is one conflict-free 16-byte read. A wavefront's scales, one dword a panel and
+// group, come through registers a group ahead.
+template <int WR, int WC, int XP, int WP, int NS, int ACT, int OCC>
 __global__ __launch_bounds__(64 * WR * WC) __attribute__((amdgpu_waves_per_eu(OCC)))
 void MxStaged(MxGemmParams p) {
   constexpr bool GATED = ACT != kPlain;
   constexpr int XT = WR * XP, WT = WC * WP;  // panels of the tile
-  static_assert(XT + WT == 4 * WR * WC && XT % 4 == 0, "four panels a wavefront");
-  static_assert(!GATED || WP % 2 == 0, "pairs of slots");
-  __shared__ __align__(16) unsigned char b0[(XT + WT) * kMxTileBytes];
-  __shared__ __align__(16) unsigned char b1[(XT + WT) * kMxTileBytes];
-  __shared__ __align__(16) unsigned char b2[(XT + WT) * kMxTileBytes];
-  __shared__ __align__(16) unsigned char b3[(XT + WT) * kMxTileBytes];
+  constexpr int ND = (XT + WT) / (WR * WC);  // panels a wavefront loads
+  static_assert(ND * WR * WC == XT + WT && WP % 2 == 0, "whole shares, pairs of slots");
+  constexpr int kStage = (XT + WT) * kMxTileBytes;
+  // One array a buffer: the compiler then sees that a tile's loads and the reads
+  // of another do not meet, and adds no wait of its own.
+  __shared__ __align__(16) unsigned char b0[kStage];
+  __shared__ __align__(16) unsigned char b1[kStage];
+  __shared__ __align__(16) unsigned char b2[kStage];
+  __shared__ __align__(16) unsigned char b3[NS > 3 ? kStage : 16];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int wr = wave / WC, wc = wave % WC;
@@ -332,35 +425,35 @@ void MxStaged(MxGemmParams p) {
   const int rt = __builtin_amdgcn_readfirstlane(4 * band + in_band % h);
   const int64_t xp0 = int64_t{rt} * XT;
   const int64_t wp0 = int64_t{ct} * (GATED ? WT / 2 : WT);
+  // Panels are a multiple of the tiles' 1 KiB apart, so with an even count of
+  // tiles the reads of one k tile meet in few of the L2's channels (256 bytes
+  // each in turn, 16 of them). Workgroups therefore take a group's tiles in
+  // different orders, tile j ^ turn at step j, the scales' bytes moved alike.
+  const uint32_t turns = p.tiles % 4 == 0 ? 3u : p.tiles % 2 == 0 ? 1u : 0u;
+  const int turn = static_cast<int>((blockIdx.x >> 3) & turns);
+  const uint32_t bytes = 0x03020100u ^ static_cast<uint32_t>(turn) * 0x01010101u;
   const int last_x = static_cast<int>(min(int64_t{XT}, p.x_panels - xp0)) - 1;
   const int last_w = static_cast<int>(min(int64_t{WT}, p.w_panels - wp0)) - 1;
 
-  // The wavefront's four panels of a stage: all of x, or all weight slots.
-  // Panels past the last read the last one: their results are not stored.
-  const int slot = 4 * wave;
-  const bool is_x = slot < XT;
+  // The wavefront's panels of a stage. Panels past the last read the last one:
+  // their results are not stored.
   const int64_t row_bytes = int64_t{p.tiles} * kMxTileBytes;
-  const uint8_t* const even = is_x ? p.xc + xp0 * row_bytes : p.wc[0] + wp0 * row_bytes;
-  const uint8_t* const odd = is_x || !GATED ? even : p.wc[1] + wp0 * row_bytes;
-  const __amdgpu_buffer_rsrc_t re = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint8_t*>(even), 0, 0xFFFFFFFFu, 0x00020000);
-  const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint8_t*>(odd), 0, 0xFFFFFFFFu, 0x00020000);
-  uint32_t src[4];
+  const uint8_t* src[ND];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int local = is_x ? min(slot + i, last_x)
-                           : min(GATED ? (slot - XT + i) / 2 : slot - XT + i, last_w);
-    src[i] = static_cast<uint32_t>(local) * static_cast<uint32_t>(row_bytes);
+  for (int i = 0; i < ND; ++i) {
+    const int slot = ND * wave + i, w = slot - XT;
+    src[i] = slot < XT ? p.xc + (xp0 + min(slot, last_x)) * row_bytes
+                       : p.wc[GATED ? w & 1 : 0] + (wp0 + min(GATED ? w / 2 : w, last_w)) * row_bytes;
   }
   auto stage = [&](unsigned char* buf, int t) __attribute__((always_inline)) {
-    const uint32_t at = static_cast<uint32_t>(min(t, p.tiles - 1)) * kMxTileBytes;
+    const uint32_t at = static_cast<uint32_t>(min(t ^ turn, p.tiles - 1)) * kMxTileBytes;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < ND; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          i & 1 ? ro : re,
-          (__attribute__((address_space(3))) void*)(buf + (slot + i) * kMxTileBytes), 16,
-          lane * 16, src[i] + at, 0, 0);
+          __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(src[i]), 0, 0xFFFFFFFFu,
+                                            0x00020000),
+          (__attribute__((address_space(3))) void*)(buf + (ND * wave + i) * kMxTileBytes), 16,
+          lane * 16, at, 0, 0);
   };
 
   // Scales of the wavefront's own panels.
@@ -397,14 +490,22 @@ void MxStaged(MxGemmParams p) {
   uint32_t sx[XP], sw[WP], nx[XP], nw[WP];
 
 #define EHIP_MX_FENCE() asm volatile("" ::: "memory")
-  load_scales(0, sx, sw);
+  auto turned = [&](const uint32_t (&ax)[XP], const uint32_t (&aw)[WP])
+                    __attribute__((always_inline)) {
+#pragma unroll
+    for (int a = 0; a < XP; ++a) sx[a] = __builtin_amdgcn_perm(0u, ax[a], bytes);
+#pragma unroll
+    for (int b = 0; b < WP; ++b) sw[b] = __builtin_amdgcn_perm(0u, aw[b], bytes);
+  };
+  load_scales(0, nx, nw);
   EHIP_MX_FENCE();
   stage(b0, 0);
   EHIP_MX_FENCE();
   stage(b1, 1);
   EHIP_MX_FENCE();
-  stage(b2, 2);
+  if constexpr (NS > 3) stage(b2, 2);
   EHIP_MX_FENCE();
+  turned(nx, nw);
   auto compute = [&](auto j, const unsigned char* buf) __attribute__((always_inline)) {
     constexpr int J = decltype(j)::value;
     i32x4_t w[WP];
@@ -420,49 +521,79 @@ void MxStaged(MxGemmParams p) {
     }
   };
   // Step t waits for its own tile's loads and meets the other wavefronts', then
-  // loads tile t + 3 into the buffer that step t - 1 has read. The loads stay
-  // unconditional (past the end: the last tile again), so that the counts
-  // hold: behind a tile's loads are two more tiles' (8), and at J = 1 and 2 the
-  // next group's XP + WP scales, which are loaded at J = 0.
-#define EHIP_MX_STEP(J, BUF, NEXT, PENDING)                                                  \
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PENDING) : "memory");      \
-  if ((J) == 0) {                                                                            \
-    load_scales(g + 1, nx, nw);                                                              \
-    EHIP_MX_FENCE();                                                                         \
-  }                                                                                          \
-  stage(NEXT, 4 * g + (J) + 3);                                                              \
-  EHIP_MX_FENCE();                                                                           \
-  compute(std::integral_constant<int, (J)>{}, BUF);                                          \
-  if (4 * g + (J) + 1 >= p.tiles) break
-  for (int g = 0;; ++g) {
-    EHIP_MX_STEP(0, b0, b3, 8);
-    EHIP_MX_STEP(1, b1, b0, 8 + XP + WP);
-    EHIP_MX_STEP(2, b2, b1, 8 + XP + WP);
-    EHIP_MX_STEP(3, b3, b2, 8);
-#pragma unroll
-    for (int a = 0; a < XP; ++a) sx[a] = nx[a];
-#pragma unroll
-    for (int b = 0; b < WP; ++b) sw[b] = nw[b];
+  // loads tile t + NS - 1 into the buffer that step t - 1 has read. The loads
+  // stay unconditional (past the end: the last tile again), so that the counts
+  // hold: behind a tile's loads are NS - 2 more tiles', and the next group's
+  // scales, which step 0 of a group loads before its tile, wherever they came in
+  // between. True after the last tile.
+  int g = 0;
+  auto step = [&](auto s) __attribute__((always_inline)) {
+    constexpr int S = decltype(s)::value, J = S % 4;
+    constexpr int kTiles = (NS - 2) * ND;
+    constexpr int kPending = J > 0 && J < NS - 1 ? kTiles + XP + WP : kTiles;
+    WaitAndMeet<kPending>();
+    if constexpr (J == 0) {
+      load_scales(g + 1, nx, nw);
+      EHIP_MX_FENCE();
+    }
+    stage(Buffer<(S + NS - 1) % NS>(b0, b1, b2, b3), 4 * g + J + NS - 1);
+    EHIP_MX_FENCE();
+    compute(std::integral_constant<int, J>{}, Buffer<S % NS>(b0, b1, b2, b3));
+    return 4 * g + J + 1 >= p.tiles;
+  };
+  auto group = [&](auto s) __attribute__((always_inline)) {
+    constexpr int S = decltype(s)::value;
+    if (step(std::integral_constant<int, S>{})) return true;
+    if (step(std::integral_constant<int, S + 1>{})) return true;
+    if (step(std::integral_constant<int, S + 2>{})) return true;
+    if (step(std::integral_constant<int, S + 3>{})) return true;
+    turned(nx, nw);
+    ++g;
+    return false;
+  };
+  for (;;) {
+    if (group(std::integral_constant<int, 0>{})) break;
+    if constexpr (NS == 3) {  // twelve steps until buffer and tile of the group meet again
+      if (group(std::integral_constant<int, 4>{})) break;
+      if (group(std::integral_constant<int, 8>{})) break;
+    }
   }
-  // Loads past the end may still be in flight: they write this workgroup's
-  // LDS, so they land before it ends.
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-#undef EHIP_MX_STEP
 #undef EHIP_MX_FENCE
 
+  // Results through LDS, so that a store instruction writes whole runs of a
+  // wavefront's columns (256 bytes a row; gated 128) instead of 64-byte pieces of
+  // 16 rows. Loads past the end may still be in flight into the buffers: they
+  // land first. A wavefront's part: PP panels' rows, 16-byte chunk c of row r at
+  // c ^ r (16 lanes of a pass hit distinct banks).
+  constexpr int C = WP * (GATED ? 2 : 4);  // chunks of a row
+  constexpr int kFit = kStage / (WR * WC) / (C * 256);
+  constexpr int PP = kFit >= 4 ? 4 : kFit >= 2 ? 2 : 1;
+  static_assert(kFit >= 1 && XP % PP == 0 && (C & (C - 1)) == 0, "whole passes");
+  unsigned char* const part = b0 + wave * (PP * C * 256);
+  WaitAndMeet<0>();
+  const int64_t col0 = (wp0 + (GATED ? wc * WP / 2 : wc * WP)) * kMxRows;
+  const int n16 = lane & 15, q = lane >> 4;
 #pragma unroll
-  for (int a = 0; a < XP; ++a) {
-    const int64_t row = (xp0 + wr * XP + a) * kMxRows + (lane & 15);
+  for (int a0 = 0; a0 < XP; a0 += PP) {
 #pragma unroll
-    for (int b = 0; b < WP; b += GATED ? 2 : 1) {
-      const int64_t panel = wp0 + (GATED ? (wc * WP + b) / 2 : wc * WP + b);
-      MxStore<ACT>(p, row, panel * kMxRows + 4 * (lane >> 4), acc[a][b],
-                     acc[a][GATED ? b + 1 : b]);
+    for (int a = 0; a < PP; ++a)
+#pragma unroll
+      for (int b = 0; b < WP; b += GATED ? 2 : 1) {
+        const int c = (GATED ? b / 2 : b) * 4 + q;
+        *reinterpret_cast<f32x4_t*>(part + ((a * 16 + n16) * C + ((c ^ n16) & (C - 1))) * 16) =
+            MxFinish<ACT>(p, col0 + 4 * c, acc[a0 + a][b], acc[a0 + a][GATED ? b + 1 : b]);
+      }
+#pragma unroll
+    for (int i = 0; i < PP * 16 * C / 64; ++i) {
+      const int r = i * (64 / C) + lane / C, c = lane % C;
+      const f32x4_t v =
+          *reinterpret_cast<const f32x4_t*>(part + (r * C + ((c ^ r) & (C - 1))) * 16);
+      MxStore(p, (xp0 + wr * XP + a0) * kMxRows + r, col0 + 4 * c, v);
     }
   }
 }
 
-template <int WR, int WC, int XP, int WP, int ACT, int OCC>
+template <int WR, int WC, int XP, int WP, int NS, int ACT, int OCC>
 hipError_t LaunchStaged(MxGemmParams p, hipStream_t stream) {
   constexpr int64_t XT = WR * XP, WT = ACT != kPlain ? WC * WP / 2 : WC * WP;
   const int64_t rt = (p.x_panels + XT - 1) / XT, ct = (p.w_panels + WT - 1) / WT;
@@ -470,28 +601,39 @@ hipError_t LaunchStaged(MxGemmParams p, hipStream_t stream) {
   p.row_tiles = static_cast<int32_t>(rt);
   p.col_tiles = static_cast<int32_t>(ct);
   const uint32_t grid = static_cast<uint32_t>((rt * ct + 7) / 8 * 8);
-  hipLaunchKernelGGL((MxStaged<WR, WC, XP, WP, ACT, OCC>), dim3(grid), dim3(64 * WR * WC), 0,
+  hipLaunchKernelGGL((MxStaged<WR, WC, XP, WP, NS, ACT, OCC>), dim3(grid), dim3(64 * WR * WC), 0,
                      stream, p);
   return hipGetLastError();
 }
 
-template <int ACT>
+template <int MP, int ACT, bool FUSED>
 hipError_t LaunchDirect(const MxGemmParams& p, hipStream_t stream) {
-  const int64_t n = p.w_panels * ((p.x_panels + 3) / 4);
+  const int64_t n = p.w_panels * ((p.x_panels + MP - 1) / MP);
   if (n > INT32_MAX) return hipErrorInvalidValue;
   const dim3 grid(static_cast<uint32_t>(n));
-  if (p.x_panels == 1)
-    hipLaunchKernelGGL((MxDirect<1, 1, ACT, 8>), grid, dim3(512), 0, stream, p);
+  // A wavefront a scale group, up to 16 (gated, with twice the operands, 8).
+  constexpr int kMost = ACT != kPlain ? 8 : 16;
+  if (kMost == 16 && p.groups > 8)
+    hipLaunchKernelGGL((MxDirect<MP, ACT, kMost, FUSED>), grid, dim3(64 * kMost), 0, stream, p);
+  else if (p.groups > 4)
+    hipLaunchKernelGGL((MxDirect<MP, ACT, 8, FUSED>), grid, dim3(512), 0, stream, p);
+  else if (p.groups > 2)
+    hipLaunchKernelGGL((MxDirect<MP, ACT, 4, FUSED>), grid, dim3(256), 0, stream, p);
   else
-    hipLaunchKernelGGL((MxDirect<4, 1, ACT, 8>), grid, dim3(512), 0, stream, p);
+    hipLaunchKernelGGL((MxDirect<MP, ACT, 2, FUSED>), grid, dim3(128), 0, stream, p);
   return hipGetLastError();
 }
 
 template <int ACT>
 hipError_t LaunchProduct(const MxGemmParams& p, hipStream_t stream) {
-  if (p.m > 256) return LaunchStaged<2, 4, 8, 4, ACT, 2>(p, stream);
-  if (p.m > 64) return LaunchStaged<2, 2, 4, 4, ACT, 2>(p, stream);
-  return LaunchDirect<ACT>(p, stream);
+  if (p.x) return LaunchDirect<1, ACT, true>(p, stream);
+  if (p.m > 64) return LaunchStaged<2, 2, 4, 4, 3, ACT, 3>(p, stream);
+  switch (p.x_panels) {
+    case 1: return LaunchDirect<1, ACT, false>(p, stream);
+    case 2: return LaunchDirect<2, ACT, false>(p, stream);
+    case 3: return LaunchDirect<3, ACT, false>(p, stream);
+    default: return LaunchDirect<4, ACT, false>(p, stream);
+  }
 }
 
 // Workgroups of the panel conversions, 0 where a launch cannot hold them.
@@ -537,6 +679,8 @@ hipError_t LaunchMxDequantize(const void* codes, const void* scales, int64_t row
                      rows, k, vec, y);
   return hipGetLastError();
 }
+
+bool MxFusesQuantization(int64_t m) { return m <= 4; }
 
 hipError_t LaunchMxGemm(const MxGemmParams& p, bool gated, hipStream_t stream) {
   if (!gated) return LaunchProduct<kPlain>(p, stream);
