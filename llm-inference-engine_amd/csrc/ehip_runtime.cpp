@@ -911,7 +911,7 @@ int RunMxGemm(ehip_ctx* ctx, const float* x, const void* xc, const void* xs, int
 // in the product's own kernel.
 int RunMxLinear(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k, const MxWeights& w,
                 int64_t n, int32_t act, float* d_y) {
-  if (ehip::MxFusesQuantization(m))
+  if (ehip::MxFusesQuantization(m, k))
     return RunMxGemm(ctx, d_x, nullptr, nullptr, m, k, w, n, act, d_y);
   const size_t codes = static_cast<size_t>(ehip::MxCodeBytes(m, k));
   if (int rc = EnsureGemmWorkspace(ctx, codes + static_cast<size_t>(ehip::MxScaleBytes(m, k))))

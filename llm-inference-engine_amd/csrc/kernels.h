@@ -275,7 +275,7 @@ struct MxGemmParams {
   int32_t row_tiles, col_tiles;  // the staged kernel's (set at its launch)
 };
 // Whether a product of m fp32 rows quantises them itself.
-bool MxFusesQuantization(int64_t m);
+bool MxFusesQuantization(int64_t m, int64_t k);
 hipError_t LaunchMxGemm(const MxGemmParams& p, bool gated, hipStream_t stream);
 
 hipError_t LaunchFillNormal(void* dst, int64_t n, int dtype, float mean, float stddev,

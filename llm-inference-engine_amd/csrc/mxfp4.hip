@@ -26,22 +26,23 @@ typedef __attribute__((ext_vector_type(4))) float f32x4_t;
 template <int DT>
 __device__ __forceinline__ void Load8(const void* x, int64_t at, float (&v)[8]) {
   if constexpr (DT == EHIP_WEIGHT_F32) {
-    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(x) + at);
-    const float4 a = p[0], b = p[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    const f32x4_t* p = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(x) + at);
+    const f32x4_t a = p[0], b = p[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
   } else {
-    const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + at);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+    const i32x4_t a = __builtin_nontemporal_load(
+        reinterpret_cast<const i32x4_t*>(static_cast<const uint16_t*>(x) + at));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      const uint32_t w = static_cast<uint32_t>(a[i]);
       if constexpr (DT == EHIP_WEIGHT_BF16) {
-        v[2 * i] = Bf16Lo(w[i]);
-        v[2 * i + 1] = Bf16Hi(w[i]);
+        v[2 * i] = Bf16Lo(w);
+        v[2 * i + 1] = Bf16Hi(w);
       } else {
-        v[2 * i] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[i])));
+        v[2 * i] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w)));
         v[2 * i + 1] =
-            static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[i] >> 16)));
+            static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w >> 16)));
       }
     }
   }
@@ -133,8 +134,9 @@ __global__ __launch_bounds__(256) void MxPack(const uint8_t* rc, const uint8_t* 
   if ((i & 3) == 0) scales[(panel * groups + group) * 64 + (i >> 2) * 16 + r] = packed;
 }
 
-// Panels into fp32 rows, over the same work split.
-__global__ __launch_bounds__(256) void MxDequantize(const uint32_t* codes, const uint32_t* scales,
+// Panels into fp32 rows. The same work split, but thread (r, i) has elements 4i
+// and 64 + 4i of a tile, so that a store instruction writes whole 256-byte runs.
+__global__ __launch_bounds__(256) void MxDequantize(const uint16_t* codes, const uint32_t* scales,
                                                     int64_t rows, int64_t k, int32_t vec,
                                                     float* y) {
   const int r = threadIdx.x >> 4, i = threadIdx.x & 15;
@@ -144,33 +146,45 @@ __global__ __launch_bounds__(256) void MxDequantize(const uint32_t* codes, const
   const int64_t panel = bp, group = blockIdx.x - bp * static_cast<uint32_t>(groups);
   const int64_t row = panel * kMxRows + r;
   if (row >= rows) return;
-  const uint32_t packed = scales[(panel * groups + group) * 64 + (i >> 2) * 16 + r];
+  // All loads first (past the last tile: the last one's), then the values.
+  uint32_t packed[2];
+  uint16_t all[kMxGroup][2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int lane = (2 * h + (i >> 3)) * 16 + r;
+    packed[h] = scales[(panel * groups + group) * 64 + lane];
+#pragma unroll
+    for (int j = 0; j < kMxGroup; ++j) {
+      const int64_t tile = min(group * kMxGroup + j, tiles - 1);
+      all[j][h] = codes[((panel * tiles + tile) * 64 + lane) * 8 + (i & 7)];
+    }
+  }
 #pragma unroll
   for (int j = 0; j < kMxGroup; ++j) {
-    const int64_t tile = group * kMxGroup + j;
-    const int64_t k0 = tile * kMxTile + 8 * i;
-    if (k0 >= k) continue;
-    const uint32_t c = codes[((panel * tiles + tile) * 64 + (i >> 2) * 16 + r) * 4 + (i & 3)];
-    const uint32_t byte = (packed >> (8 * j)) & 255u;
-    float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      // E2M1 as fp32: exponent 0 is m / 2, the others 2^(exponent - 1) (1 + m / 2).
-      const uint32_t code = (c >> (4 * e)) & 15u, m = code & 7u;
-      const float mag = m < 2u ? 0.5f * static_cast<float>(m)
-                               : __uint_as_float((126u + (m >> 1)) << 23 | (m & 1u) << 22);
-      const float s = code & 8u ? -mag : mag;
-      v[e] = byte == 255u ? __builtin_nanf("")
-                          : __builtin_amdgcn_ldexpf(s, static_cast<int>(byte) - 127);
-    }
-    float* out = y + row * k + k0;
-    if (vec && k0 + 8 <= k) {
-      reinterpret_cast<float4*>(out)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(out)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
+    for (int h = 0; h < 2; ++h) {
+      const int64_t k0 = (group * kMxGroup + j) * kMxTile + 64 * h + 4 * i;
+      if (k0 >= k) continue;
+      const uint32_t byte = (packed[h] >> (8 * j)) & 255u;
+      f32x4_t v;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (k0 + e < k) out[e] = v[e];
+      for (int e = 0; e < 4; ++e) {
+        // E2M1 as fp32: exponent 0 is m / 2, the others 2^(exponent - 1) (1 + m / 2).
+        const uint32_t code = (uint32_t{all[j][h]} >> (4 * e)) & 15u, m = code & 7u;
+        const float mag = m < 2u ? 0.5f * static_cast<float>(m)
+                                 : __uint_as_float((126u + (m >> 1)) << 23 | (m & 1u) << 22);
+        const float s = code & 8u ? -mag : mag;
+        v[e] = byte == 255u ? __builtin_nanf("")
+                            : __builtin_amdgcn_ldexpf(s, static_cast<int>(byte) - 127);
+      }
+      float* out = y + row * k + k0;
+      if (vec) {  // k % 4 == 0
+        __builtin_nontemporal_store(v, reinterpret_cast<f32x4_t*>(out));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (k0 + e < k) out[e] = v[e];
+      }
     }
   }
 }
@@ -226,29 +240,11 @@ __device__ __forceinline__ void MxStore(const MxGemmParams& p, int64_t row, int6
   }
 }
 
-// 32 values of one block as codes and the scale byte.
-__device__ __forceinline__ i32x4_t MxBlock(const f32x4_t (&v)[8], uint32_t* byte) {
-  float top = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) top = __builtin_elementwise_maximum(top, fabsf(v[i][e]));
-  *byte = MxScaleByte(__float_as_uint(top) & 0x7FFFFFFFu);
-  i32x4_t codes;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float w[8] = {v[2 * i][0],     v[2 * i][1],     v[2 * i][2],     v[2 * i][3],
-                        v[2 * i + 1][0], v[2 * i + 1][1], v[2 * i + 1][2], v[2 * i + 1][3]};
-    codes[i] = static_cast<int>(MxCodes(w, *byte));
-  }
-  return codes;
-}
-
 // Few rows: a workgroup per (MP x panels, one weight panel a projection), its KW
 // wavefronts taking the scale groups in turn with their operands straight from
 // memory into registers, a group ahead, then one sum over the wavefronts through
-// LDS, in their order. FUSED (MP = 1): x is fp32 rows, and a lane quantises its
-// own block.
+// LDS, in their order. FUSED (MP = 1): x is fp32 rows, which the workgroup
+// quantises into LDS while its first weights are on their way.
 template <int MP, int ACT, int KW, bool FUSED>
 __global__ __launch_bounds__(64 * KW) void MxDirect(MxGemmParams p) {
   static_assert(!FUSED || MP == 1, "fused quantisation of one panel");
@@ -282,7 +278,10 @@ __global__ __launch_bounds__(64 * KW) void MxDirect(MxGemmParams p) {
   }
   const int row = lane & 15, block = lane >> 4;
   const bool live = row < p.m;
-  const float* const xf = FUSED ? p.x + int64_t{live ? row : 0} * p.k : nullptr;
+  // FUSED: codes [m][groups][16 blocks][16 bytes], then scales [m][groups][64
+  // bytes] in the panels' order within a row (byte j of dword g).
+  extern __shared__ __align__(16) uint32_t quant[];
+  const int x_dwords = FUSED ? static_cast<int>(p.m) * p.groups * 64 : 0;
 
   i32x4_t x[kMxGroup][MP], w[kMxGroup][PR];
   uint32_t sx[MP], sw[PR];
@@ -308,33 +307,45 @@ __global__ __launch_bounds__(64 * KW) void MxDirect(MxGemmParams p) {
 #pragma unroll
     for (int j = 0; j < kMxGroup; ++j) load(wave, j);
   }
+  if constexpr (FUSED) {
+    // Four threads a block, eight values each; blocks past k are zeros.
+    for (int c = threadIdx.x; c < x_dwords; c += 64 * KW) {
+      const int r = c / (p.groups * 64), in_row = c - r * (p.groups * 64);
+      const int64_t k0 = int64_t{in_row} * 8;
+      const float* src = p.x + r * p.k + k0;
+      float v[8];
+      if (p.x_vec && k0 + 8 <= p.k) {
+        const f32x4_t a = reinterpret_cast<const f32x4_t*>(src)[0];
+        const f32x4_t b = reinterpret_cast<const f32x4_t*>(src)[1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = k0 + e < p.k ? src[e] : 0.f;
+      }
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+      const uint32_t byte = MxScaleByte(DppMax4(top));
+      quant[c] = MxCodes(v, byte);
+      const int blk = in_row / 4;  // in the row: group blk / 16, tile blk / 4 % 4, block blk % 4
+      if ((c & 3) == 0)
+        reinterpret_cast<uint8_t*>(quant + x_dwords)[((r * p.groups + blk / 16) * 4 + blk % 4) * 4 +
+                                                     blk / 4 % 4] = static_cast<uint8_t>(byte);
+    }
+    __syncthreads();
+  }
   for (int t = wave; t < p.groups; t += KW) {
     uint32_t cx[MP], cw[PR];
 #pragma unroll
     for (int b = 0; b < PR; ++b) cw[b] = sw[b];
     if constexpr (FUSED) {
-      // The codes of the group's blocks; byte j of the scales is tile j's.
-      cx[0] = 0;
 #pragma unroll
-      for (int j = 0; j < kMxGroup; ++j) {
-        const int64_t k0 = (int64_t{t} * kMxGroup + j) * kMxTile + block * kMxBlock;
-        f32x4_t v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        if (live && p.x_vec && k0 + kMxBlock <= p.k) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const f32x4_t*>(xf + k0 + 4 * i);
-        } else if (live) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (k0 + 4 * i + e < p.k) v[i][e] = xf[k0 + 4 * i + e];
-        }
-        uint32_t byte;
-        x[j][0] = MxBlock(v, &byte);
-        cx[0] |= byte << (8 * j);
-      }
+      for (int j = 0; j < kMxGroup; ++j)
+        x[j][0] = live ? *reinterpret_cast<const i32x4_t*>(
+                             quant + ((row * p.groups + t) * 16 + 4 * j + block) * 4)
+                       : i32x4_t{0, 0, 0, 0};
+      cx[0] = live ? quant[x_dwords + (row * p.groups + t) * 4 + block] : 0u;
     } else {
 #pragma unroll
       for (int a = 0; a < MP; ++a) cx[a] = sx[a];
@@ -393,18 +404,25 @@ __device__ __forceinline__ void WaitAndMeet() {
 // projection's). k tiles go from memory straight into LDS (buffer_load ... lds, a
 // panel's 1 KiB an instruction), into NS buffers, NS - 1 tiles ahead; an operand
 // is one conflict-free 16-byte read. A wavefront's scales, one dword a panel and
-// group, come through registers a group ahead.
-template <int WR, int WC, int XP, int WP, int NS, int ACT, int OCC>
+// group, come through registers a group ahead. WD > 0 (WR = 1, where no two
+// wavefronts share a weight panel): the weights go into registers instead, WD - 1
+// tiles ahead, which takes half of the traffic off LDS.
+template <int WR, int WC, int XP, int WP, int NS, int WD, int ACT, int OCC>
 __global__ __launch_bounds__(64 * WR * WC) __attribute__((amdgpu_waves_per_eu(OCC)))
 void MxStaged(MxGemmParams p) {
   constexpr bool GATED = ACT != kPlain;
   constexpr int XT = WR * XP, WT = WC * WP;  // panels of the tile
-  constexpr int ND = (XT + WT) / (WR * WC);  // panels a wavefront loads
-  static_assert(ND * WR * WC == XT + WT && WP % 2 == 0, "whole shares, pairs of slots");
-  constexpr int kStage = (XT + WT) * kMxTileBytes;
+  constexpr int LT = XT + (WD ? 0 : WT);  // of them through LDS
+  constexpr int ND = LT / (WR * WC);      // panels a wavefront loads into it
+  static_assert(ND * WR * WC == LT && WP % 2 == 0, "whole shares, pairs of slots");
+  static_assert(WD == 0 || (WR == 1 && NS == 4 && (WD == 2 || WD == 4)), "register tiles");
+  constexpr int kStage = LT * kMxTileBytes;
+  constexpr int C = WP * (GATED ? 2 : 4);  // 16-byte chunks of a wavefront's row of results
+  constexpr int kResults = WR * WC * C * 256;
+  constexpr int kFirst = kStage > kResults ? kStage : kResults;
   // One array a buffer: the compiler then sees that a tile's loads and the reads
   // of another do not meet, and adds no wait of its own.
-  __shared__ __align__(16) unsigned char b0[kStage];
+  __shared__ __align__(16) unsigned char b0[kFirst];
   __shared__ __align__(16) unsigned char b1[kStage];
   __shared__ __align__(16) unsigned char b2[kStage];
   __shared__ __align__(16) unsigned char b3[NS > 3 ? kStage : 16];
@@ -445,6 +463,24 @@ void MxStaged(MxGemmParams p) {
     src[i] = slot < XT ? p.xc + (xp0 + min(slot, last_x)) * row_bytes
                        : p.wc[GATED ? w & 1 : 0] + (wp0 + min(GATED ? w / 2 : w, last_w)) * row_bytes;
   }
+  const uint8_t* wsrc[WD ? WP : 1];
+#pragma unroll
+  for (int b = 0; b < (WD ? WP : 0); ++b) {
+    const int w = wc * WP + b;
+    wsrc[b] = p.wc[GATED ? w & 1 : 0] + (wp0 + min(GATED ? w / 2 : w, last_w)) * row_bytes;
+  }
+  constexpr int kW = WD ? WD : 1;
+  i32x4_t wf[kW][WP];
+  auto load_w = [&](i32x4_t (&w)[WP], int t) __attribute__((always_inline)) {
+    const uint32_t at = static_cast<uint32_t>(min(t ^ turn, p.tiles - 1)) * kMxTileBytes;
+#pragma unroll
+    for (int b = 0; b < (WD ? WP : 0); ++b)
+      w[b] = __builtin_bit_cast(
+          i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                       __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(wsrc[b]), 0,
+                                                         0xFFFFFFFFu, 0x00020000),
+                       lane * 16, at, 0));
+  };
   auto stage = [&](unsigned char* buf, int t) __attribute__((always_inline)) {
     const uint32_t at = static_cast<uint32_t>(min(t ^ turn, p.tiles - 1)) * kMxTileBytes;
 #pragma unroll
@@ -500,17 +536,20 @@ void MxStaged(MxGemmParams p) {
   load_scales(0, nx, nw);
   EHIP_MX_FENCE();
   stage(b0, 0);
+  if constexpr (WD > 0) load_w(wf[0], 0);
   EHIP_MX_FENCE();
   stage(b1, 1);
+  if constexpr (WD > 2) load_w(wf[1], 1);
   EHIP_MX_FENCE();
   if constexpr (NS > 3) stage(b2, 2);
+  if constexpr (WD > 2) load_w(wf[2], 2);
   EHIP_MX_FENCE();
   turned(nx, nw);
-  auto compute = [&](auto j, const unsigned char* buf) __attribute__((always_inline)) {
+  auto compute = [&](auto j, const unsigned char* buf, i32x4_t (&w)[WP])
+                     __attribute__((always_inline)) {
     constexpr int J = decltype(j)::value;
-    i32x4_t w[WP];
 #pragma unroll
-    for (int b = 0; b < WP; ++b)
+    for (int b = 0; b < (WD ? 0 : WP); ++b)
       w[b] = *reinterpret_cast<const i32x4_t*>(buf + (XT + wc * WP + b) * kMxTileBytes + lane * 16);
 #pragma unroll
     for (int a = 0; a < XP; ++a) {
@@ -523,13 +562,13 @@ void MxStaged(MxGemmParams p) {
   // Step t waits for its own tile's loads and meets the other wavefronts', then
   // loads tile t + NS - 1 into the buffer that step t - 1 has read. The loads
   // stay unconditional (past the end: the last tile again), so that the counts
-  // hold: behind a tile's loads are NS - 2 more tiles', and the next group's
-  // scales, which step 0 of a group loads before its tile, wherever they came in
-  // between. True after the last tile.
+  // hold: behind a tile's loads are NS - 2 more tiles', WD - 1 or more sets of
+  // weights, and the next group's scales, which step 0 of a group loads before
+  // its tile, wherever they came in between. True after the last tile.
   int g = 0;
   auto step = [&](auto s) __attribute__((always_inline)) {
     constexpr int S = decltype(s)::value, J = S % 4;
-    constexpr int kTiles = (NS - 2) * ND;
+    constexpr int kTiles = (NS - 2) * ND + (WD ? WD - 1 : 0) * WP;
     constexpr int kPending = J > 0 && J < NS - 1 ? kTiles + XP + WP : kTiles;
     WaitAndMeet<kPending>();
     if constexpr (J == 0) {
@@ -537,8 +576,10 @@ void MxStaged(MxGemmParams p) {
       EHIP_MX_FENCE();
     }
     stage(Buffer<(S + NS - 1) % NS>(b0, b1, b2, b3), 4 * g + J + NS - 1);
+    if constexpr (WD > 0) load_w(wf[(S + WD - 1) % kW], 4 * g + J + WD - 1);
     EHIP_MX_FENCE();
-    compute(std::integral_constant<int, J>{}, Buffer<S % NS>(b0, b1, b2, b3));
+    compute(std::integral_constant<int, J>{}, Buffer<S % NS>(b0, b1, b2, b3),
+            wf[S % kW]);
     return 4 * g + J + 1 >= p.tiles;
   };
   auto group = [&](auto s) __attribute__((always_inline)) {
@@ -565,8 +606,7 @@ void MxStaged(MxGemmParams p) {
   // 16 rows. Loads past the end may still be in flight into the buffers: they
   // land first. A wavefront's part: PP panels' rows, 16-byte chunk c of row r at
   // c ^ r (16 lanes of a pass hit distinct banks).
-  constexpr int C = WP * (GATED ? 2 : 4);  // chunks of a row
-  constexpr int kFit = kStage / (WR * WC) / (C * 256);
+  constexpr int kFit = kFirst / kResults;
   constexpr int PP = kFit >= 4 ? 4 : kFit >= 2 ? 2 : 1;
   static_assert(kFit >= 1 && XP % PP == 0 && (C & (C - 1)) == 0, "whole passes");
   unsigned char* const part = b0 + wave * (PP * C * 256);
@@ -593,7 +633,7 @@ void MxStaged(MxGemmParams p) {
   }
 }
 
-template <int WR, int WC, int XP, int WP, int NS, int ACT, int OCC>
+template <int WR, int WC, int XP, int WP, int NS, int WD, int ACT, int OCC>
 hipError_t LaunchStaged(MxGemmParams p, hipStream_t stream) {
   constexpr int64_t XT = WR * XP, WT = ACT != kPlain ? WC * WP / 2 : WC * WP;
   const int64_t rt = (p.x_panels + XT - 1) / XT, ct = (p.w_panels + WT - 1) / WT;
@@ -601,7 +641,7 @@ hipError_t LaunchStaged(MxGemmParams p, hipStream_t stream) {
   p.row_tiles = static_cast<int32_t>(rt);
   p.col_tiles = static_cast<int32_t>(ct);
   const uint32_t grid = static_cast<uint32_t>((rt * ct + 7) / 8 * 8);
-  hipLaunchKernelGGL((MxStaged<WR, WC, XP, WP, NS, ACT, OCC>), dim3(grid), dim3(64 * WR * WC), 0,
+  hipLaunchKernelGGL((MxStaged<WR, WC, XP, WP, NS, WD, ACT, OCC>), dim3(grid), dim3(64 * WR * WC), 0,
                      stream, p);
   return hipGetLastError();
 }
@@ -611,29 +651,49 @@ hipError_t LaunchDirect(const MxGemmParams& p, hipStream_t stream) {
   const int64_t n = p.w_panels * ((p.x_panels + MP - 1) / MP);
   if (n > INT32_MAX) return hipErrorInvalidValue;
   const dim3 grid(static_cast<uint32_t>(n));
+  const uint32_t lds = FUSED ? static_cast<uint32_t>(p.m * p.groups) * 272u : 0u;
   // A wavefront a scale group, up to 16 (gated, with twice the operands, 8).
   constexpr int kMost = ACT != kPlain ? 8 : 16;
   if (kMost == 16 && p.groups > 8)
-    hipLaunchKernelGGL((MxDirect<MP, ACT, kMost, FUSED>), grid, dim3(64 * kMost), 0, stream, p);
+    hipLaunchKernelGGL((MxDirect<MP, ACT, kMost, FUSED>), grid, dim3(64 * kMost), lds, stream, p);
   else if (p.groups > 4)
-    hipLaunchKernelGGL((MxDirect<MP, ACT, 8, FUSED>), grid, dim3(512), 0, stream, p);
+    hipLaunchKernelGGL((MxDirect<MP, ACT, 8, FUSED>), grid, dim3(512), lds, stream, p);
   else if (p.groups > 2)
-    hipLaunchKernelGGL((MxDirect<MP, ACT, 4, FUSED>), grid, dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((MxDirect<MP, ACT, 4, FUSED>), grid, dim3(256), lds, stream, p);
   else
-    hipLaunchKernelGGL((MxDirect<MP, ACT, 2, FUSED>), grid, dim3(128), 0, stream, p);
+    hipLaunchKernelGGL((MxDirect<MP, ACT, 2, FUSED>), grid, dim3(128), lds, stream, p);
   return hipGetLastError();
 }
 
+// Which kernel, by how many workgroups of each there are (us, this kernel / the
+// next one tried, four weight sets in turn):
+//   direct, up to 64 rows or 512 workgroups (two a CU): 96 x 4096 x 4096 6.3 / 8.4,
+//     128 x 16384 x 4096 20 / 24; past it 200 x 4096 x 4096 10.1 / 8.9.
+//   64 x 64 tiles, up to 896 (3.5 a CU): 512 x 4096 x 4096 11.1 / 15.5, gated 500 x
+//     896 x 3584 6.9 / 7.8; past it 1024 x 4096 x 4096 20.0 / 17.5.
+//   128 x 256 tiles with the weights in registers, from 448 of them (1.75 a CU)
+//     over 16 k tiles and more: gated 4001 x 4096 x 16384 288 / 307, 512 rows 42.3 /
+//     45.3; below, 2382 x 4096 x 4096 34.3 / 30.7, and gated 4001 x 896 x 3584 28.1
+//     / 26.2.
+//   128 x 128 tiles, three workgroups a CU, between.
 template <int ACT>
 hipError_t LaunchProduct(const MxGemmParams& p, hipStream_t stream) {
   if (p.x) return LaunchDirect<1, ACT, true>(p, stream);
-  if (p.m > 64) return LaunchStaged<2, 2, 4, 4, 3, ACT, 3>(p, stream);
-  switch (p.x_panels) {
-    case 1: return LaunchDirect<1, ACT, false>(p, stream);
-    case 2: return LaunchDirect<2, ACT, false>(p, stream);
-    case 3: return LaunchDirect<3, ACT, false>(p, stream);
-    default: return LaunchDirect<4, ACT, false>(p, stream);
+  const int64_t slots = p.w_panels * (ACT != kPlain ? 2 : 1);
+  auto tiles = [&](int64_t x, int64_t w) {
+    return (p.x_panels + x - 1) / x * ((slots + w - 1) / w);
+  };
+  if (p.x_panels <= 4 || (p.x_panels + 3) / 4 * p.w_panels <= 512) {
+    switch (p.x_panels) {
+      case 1: return LaunchDirect<1, ACT, false>(p, stream);
+      case 2: return LaunchDirect<2, ACT, false>(p, stream);
+      case 3: return LaunchDirect<3, ACT, false>(p, stream);
+      default: return LaunchDirect<4, ACT, false>(p, stream);
+    }
   }
+  if (tiles(4, 4) <= 896) return LaunchStaged<2, 2, 2, 2, 4, 0, ACT, 4>(p, stream);
+  if (tiles(8, 16) >= 448 && p.tiles >= 16) return LaunchStaged<1, 4, 8, 4, 4, 2, ACT, 2>(p, stream);
+  return LaunchStaged<2, 2, 4, 4, 3, 0, ACT, 3>(p, stream);
 }
 
 // Workgroups of the panel conversions, 0 where a launch cannot hold them.
@@ -672,15 +732,15 @@ hipError_t LaunchMxPack(const uint8_t* row_codes, const uint8_t* row_scales, int
 hipError_t LaunchMxDequantize(const void* codes, const void* scales, int64_t rows, int64_t k,
                               float* y, hipStream_t stream) {
   const dim3 grid(MxConvertGrid(rows, k));
-  const int32_t vec = k % 8 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+  const int32_t vec = k % 4 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
   if (grid.x == 0) return hipErrorInvalidValue;
   hipLaunchKernelGGL(MxDequantize, grid, dim3(256), 0, stream,
-                     static_cast<const uint32_t*>(codes), static_cast<const uint32_t*>(scales),
+                     static_cast<const uint16_t*>(codes), static_cast<const uint32_t*>(scales),
                      rows, k, vec, y);
   return hipGetLastError();
 }
 
-bool MxFusesQuantization(int64_t m) { return m <= 4; }
+bool MxFusesQuantization(int64_t m, int64_t k) { return m <= 4 && m * MxGroups(k) * 272 <= 32768; }
 
 hipError_t LaunchMxGemm(const MxGemmParams& p, bool gated, hipStream_t stream) {
   if (!gated) return LaunchProduct<kPlain>(p, stream);
