@@ -801,26 +801,7 @@ int ehip_pack_weight_panels(ehip_ctx* ctx, const void* d_w, int32_t weight_dtype
 }
 
 namespace {
-
-// The planned linear layer (or gated block) with its workspace: x's bf16
-// planes, then (split k) the partial sums, 256 bytes apart.
-int RunPackedGemm(ehip_ctx* ctx, ehip::GemmParams& p, const float* d_x, int64_t m, int64_t k,
-                  int32_t weight_dtype, int64_t n, float* d_y, bool gated) {
-  ehip::PlanPackedGemm(m, k, n, weight_dtype, ctx->cus, &p, gated);
-  p.x = d_x;
-  p.y = d_y;
-  p.x_vec = (k % 4 == 0 && reinterpret_cast<uintptr_t>(d_x) % 16 == 0) ? 1 : 0;
-  const size_t planes = Align256(ehip::PackedGemmPlaneBytes(p));
-  if (int rc = EnsureGemmWorkspace(ctx, planes + ehip::PackedGemmPartBytes(p))) return rc;
-  p.xp = reinterpret_cast<uint16_t*>(ctx->d_gemm);
-  p.part = p.splits > 1 ? reinterpret_cast<float*>(reinterpret_cast<char*>(ctx->d_gemm) + planes)
-                        : nullptr;
-  EHIP_HIP(ctx, ehip::LaunchPackedGemm(p, weight_dtype, ctx->stream));
-  return EHIP_OK;
-}
-
 bool Aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
-
 }  // namespace
 
 int ehip_packed_gemm(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k, const void* d_wp,
@@ -840,9 +821,20 @@ int ehip_packed_gemm(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k, cons
     return SetError(ctx, EHIP_INVALID_ARGUMENT,
                     "gemm: the packed weight must be 16-byte aligned (ehip_malloc gives 256)");
   ehip::GemmParams p{};
+  ehip::PlanPackedGemm(m, k, n, weight_dtype, ctx->cus, &p);
+  p.x = d_x;
   p.wp = d_wp;
   p.bias = d_bias;
-  return RunPackedGemm(ctx, p, d_x, m, k, weight_dtype, n, d_y, false);
+  p.y = d_y;
+  p.x_vec = (k % 4 == 0 && Aligned(d_x, 16)) ? 1 : 0;
+  // x's bf16 planes, then (split k) the partial sums, 256 bytes apart.
+  const size_t planes = Align256(ehip::PackedGemmPlaneBytes(p));
+  if (int rc = EnsureGemmWorkspace(ctx, planes + ehip::PackedGemmPartBytes(p))) return rc;
+  p.xp = reinterpret_cast<uint16_t*>(ctx->d_gemm);
+  p.part = p.splits > 1 ? reinterpret_cast<float*>(reinterpret_cast<char*>(ctx->d_gemm) + planes)
+                        : nullptr;
+  EHIP_HIP(ctx, ehip::LaunchPackedGemm(p, weight_dtype, ctx->stream));
+  return EHIP_OK;
 }
 
 // ------------------------------------------------- feed-forward operators --
@@ -1020,13 +1012,21 @@ int ehip_packed_gated_gemm(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k
   if (!Aligned(d_wp_gate, 16) || !Aligned(d_wp_up, 16))
     return SetError(ctx, EHIP_INVALID_ARGUMENT,
                     "gated gemm: the packed weights must be 16-byte aligned (ehip_malloc gives 256)");
-  ehip::GemmParams p{};
-  p.wp = d_wp_gate;
-  p.wp2 = d_wp_up;
-  p.bias = d_bias_gate;
-  p.bias2 = d_bias_up;
+  ehip::GatedParams p{};
+  if (int rc = EnsureGemmWorkspace(ctx, ehip::PlanGatedGemm(m, k, n, weight_dtype, &p))) return rc;
+  p.x = d_x;
+  p.wp[0] = d_wp_gate;
+  p.wp[1] = d_wp_up;
+  p.bias[0] = d_bias_gate;
+  p.bias[1] = d_bias_up;
+  p.y = d_y;
+  p.xp = reinterpret_cast<uint16_t*>(ctx->d_gemm);
+  p.row_scale = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(ctx->d_gemm) + p.scale_at);
+  p.x_vec = k % 4 == 0 && Aligned(d_x, 16);
+  p.y_vec = n % 4 == 0 && Aligned(d_y, 16);
   p.act = activation;
-  return RunPackedGemm(ctx, p, d_x, m, k, weight_dtype, n, d_y, true);
+  EHIP_HIP(ctx, ehip::LaunchGatedGemm(p, weight_dtype, ctx->stream));
+  return EHIP_OK;
 }
 
 namespace {

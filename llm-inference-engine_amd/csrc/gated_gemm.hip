@@ -1,0 +1,679 @@
+// The gated feed-forward block over packed weights, both projections, the
+// activation and the product in one kernel:
+//   y[m, n] = act(x Wg^T + bg) * (x Wu^T + bu),
+// x fp32, the weights fp32, bf16 or fp16 in panels [ceil(n/16), k, 16].
+//
+// Two kernels. GatedStream, for a few rows, reads the panels once and multiplies
+// in fp32 on the vector ALUs. GatedStaged, for more, is on the matrix cores: x is
+// cut into 16-bit planes whose sum is the value to 2^-24 (three of bf16; beside
+// fp16 weights two of fp16, after a power of two per row that brings the row's
+// largest magnitude to 2^14), the weights as they are (bf16, fp16) or in three
+// bf16 planes (fp32). Products x_i w_j with i + j <= 2, smallest first, fp32 sums:
+// three matrix-core products a term for bf16 weights, two for fp16, six for
+// fp32. What is left out is below 2^-24 of |x||w| a term (fp16: and of 2^-39 of the
+// row's largest |x| times |w|).
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <type_traits>
+
+#include "kernels.h"
+#include "staged.h"
+
+namespace ehip {
+namespace {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
+typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4_t;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
+typedef __attribute__((ext_vector_type(4))) short s16x4_t;
+typedef __attribute__((ext_vector_type(8))) short s16x8_t;
+
+constexpr int kStreamRows = 8;     // up to these: GatedStream
+constexpr int kDirectPanels = 16;  // up to these, fp32 weights: GatedDirect
+
+constexpr int kRows = 16;   // rows of a panel, of x or a weight
+constexpr int kStep = 32;   // k of a step
+
+template <int WT>
+struct Type;
+template <>
+struct Type<EHIP_WEIGHT_F32> {
+  using T = float;
+  static constexpr int XPL = 3, WPL = 3;  // planes of x and of a weight
+};
+template <>
+struct Type<EHIP_WEIGHT_BF16> {
+  using T = uint16_t;
+  static constexpr int XPL = 3, WPL = 1;
+};
+template <>
+struct Type<EHIP_WEIGHT_F16> {
+  using T = uint16_t;
+  static constexpr int XPL = 2, WPL = 1;
+};
+
+// A lane (n16, q) of a matrix-core operand holds eight k of a 32-k step: 4q..4q+3
+// and 16+4q..16+4q+3, what two transposed LDS reads of 16-bit panel rows give;
+// q, q+4, .. q+28 for fp32 panel rows, whose single reads then meet no bank twice.
+template <int WT>
+__device__ __forceinline__ int OperandK(int q, int e) {
+  return WT == EHIP_WEIGHT_F32 ? q + 4 * e : 4 * q + (e & 3) + 16 * (e >> 2);
+}
+
+// v cut into planes: each the nearest 16-bit value of what the earlier ones leave.
+template <int WT>
+__device__ __forceinline__ void Cut(float v, short (&out)[Type<WT>::XPL]) {
+#pragma unroll
+  for (int i = 0; i < Type<WT>::XPL; ++i) {
+    if constexpr (WT == EHIP_WEIGHT_F16) {
+      const _Float16 h = static_cast<_Float16>(v);
+      out[i] = __builtin_bit_cast(short, h);
+      v -= static_cast<float>(h);
+    } else {
+      const __bf16 h = static_cast<__bf16>(v);
+      out[i] = __builtin_bit_cast(short, h);
+      v -= static_cast<float>(h);
+    }
+  }
+}
+
+// x [m, k] into operand panels [panels][steps][planes][64 lanes][8]: zero past m
+// and k. A workgroup takes a panel's steps [chunk * blockIdx.y, ..), a wavefront a
+// step at a time; for fp16 every workgroup of a panel first finds its rows'
+// largest magnitudes.
+template <int WT>
+__global__ __launch_bounds__(256) void CutRows(GatedParams p, int chunk) {
+  constexpr int PL = Type<WT>::XPL;
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const int64_t panel = blockIdx.x, row = panel * kRows + r;
+  const float* const src = p.x + (row < p.m ? row : 0) * p.k;
+  int up = 0;
+  if constexpr (WT == EHIP_WEIGHT_F16) {
+    // 16 threads a row. As integers: the order of non-negative floats, NaN and
+    // infinities on top (such a row is left as it is).
+    __shared__ int scale[kRows];
+    const int mine = threadIdx.x >> 4, i = threadIdx.x & 15;
+    const int64_t at = panel * kRows + mine;
+    uint32_t top = 0;
+    if (at < p.m) {
+      const float* const from = p.x + at * p.k;
+      int64_t kk = 0;
+      if (p.x_vec) {
+#pragma unroll 4
+        for (kk = 4 * i; kk + 4 <= p.k; kk += 64) {
+          const f32x4_t a = *reinterpret_cast<const f32x4_t*>(from + kk);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(a[e]) & 0x7FFFFFFFu);
+        }
+      } else {
+#pragma unroll 4
+        for (kk = i; kk < p.k; kk += 16) top = max(top, __float_as_uint(from[kk]) & 0x7FFFFFFFu);
+      }
+    }
+    top = max(top, static_cast<uint32_t>(
+                       __builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0xB1, 0xF, 0xF, false)));
+    top = max(top, static_cast<uint32_t>(
+                       __builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0x4E, 0xF, 0xF, false)));
+    top = max(top, static_cast<uint32_t>(
+                       __builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0x141, 0xF, 0xF, false)));
+    top = max(top, static_cast<uint32_t>(
+                       __builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0x128, 0xF, 0xF, false)));
+    const int f = static_cast<int>(top >> 23);
+    if (i == 0) scale[mine] = f == 255 ? 0 : 14 + 127 - f;
+    __syncthreads();
+    up = scale[r];
+    if (blockIdx.y == 0 && threadIdx.x < kRows) p.row_scale[row] = -up;
+  }
+  const int64_t s0 = int64_t{blockIdx.y} * chunk, s1 = min(s0 + chunk, p.steps);
+  for (int64_t s = s0 + (threadIdx.x >> 6); s < s1; s += 4) {
+    float v[8];
+    if constexpr (WT == EHIP_WEIGHT_F32) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int64_t kk = s * kStep + OperandK<WT>(q, e);
+        v[e] = row < p.m && kk < p.k ? src[kk] : 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t kk = s * kStep + 16 * h + 4 * q;
+        if (p.x_vec && row < p.m && kk + 4 <= p.k) {
+          const f32x4_t a = *reinterpret_cast<const f32x4_t*>(src + kk);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[4 * h + e] = a[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[4 * h + e] = row < p.m && kk + e < p.k ? src[kk + e] : 0.f;
+        }
+      }
+    }
+    s16x8_t out[PL];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      short parts[PL];
+      if constexpr (WT == EHIP_WEIGHT_F16)
+        Cut<WT>(__builtin_amdgcn_ldexpf(v[e], up), parts);
+      else
+        Cut<WT>(v[e], parts);
+#pragma unroll
+      for (int i = 0; i < PL; ++i) out[i][e] = parts[i];
+    }
+#pragma unroll
+    for (int i = 0; i < PL; ++i)
+      reinterpret_cast<s16x8_t*>(p.xp)[((panel * p.steps + s) * PL + i) * 64 + lane] = out[i];
+  }
+}
+
+// ds_read_b64_tr_b16: lane i of each 16-lane group receives element i % 4 of
+// the 8 bytes addressed by lanes 4j + i / 4 of the group, for j = 0..3.
+__device__ __forceinline__ s16x4_t TransposedRead(const unsigned char* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(p));
+}
+
+template <int WT>
+__device__ __forceinline__ f32x4_t Mfma(s16x8_t w, s16x8_t x, f32x4_t acc) {
+  if constexpr (WT == EHIP_WEIGHT_F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w),
+                                                  __builtin_bit_cast(f16x8_t, x), acc, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w),
+                                                   __builtin_bit_cast(bf16x8_t, x), acc, 0, 0, 0);
+}
+
+// One KiB of every step that a wavefront brings into LDS: from src + t stride
+// (zeros past `size` bytes) to `at` of the step's buffer.
+struct Unit {
+  const unsigned char* src;
+  uint32_t size, stride, at;
+};
+__device__ __forceinline__ void LoadUnit(const Unit& u, unsigned char* buf, uint32_t t, int lane) {
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<unsigned char*>(u.src), 0, u.size, 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      r, (__attribute__((address_space(3))) void*)(buf + u.at), 16, lane * 16 + t * u.stride, 0, 0,
+      0);
+}
+
+// A workgroup of WR x WC wavefronts per tile of WR XP panels of x by WC WP weight
+// slots (slot 2j the gate's panel j, 2j + 1 the up projection's). A step's x
+// planes and panel rows go from memory straight into LDS (buffer_load ... lds, 1
+// KiB units shared out over the wavefronts), NS - 1 steps
+// ahead. The weight is the A operand and x the B operand: a lane's four results
+// are four columns of one row of y.
+template <int WT, int WR, int WC, int XP, int WP, int NS, int ACT, int OCC>
+__global__ __launch_bounds__(64 * WR * WC) __attribute__((amdgpu_waves_per_eu(OCC)))
+void GatedStaged(GatedParams p) {
+  using T = typename Type<WT>::T;
+  constexpr int XPL = Type<WT>::XPL, WPL = Type<WT>::WPL, WU = sizeof(T) / 2;
+  constexpr int XT = WR * XP, SL = WC * WP;     // panels of x, weight slots of the tile
+  constexpr int kXUnits = XT * XPL, kUnits = kXUnits + SL * WU;
+  constexpr int ND = (kUnits + WR * WC - 1) / (WR * WC);  // units a wavefront loads
+  constexpr int kStage = kUnits * 1024, C = WP * 2;
+  constexpr int kResults = WR * WC * C * 256;
+  constexpr int kFirst = kStage > kResults ? kStage : kResults;
+  __shared__ __align__(16) unsigned char b0[kFirst];
+  __shared__ __align__(16) unsigned char b1[kStage];
+  __shared__ __align__(16) unsigned char b2[NS > 2 ? kStage : 16];
+  __shared__ __align__(16) unsigned char b3[NS > 3 ? kStage : 16];
+  const int lane = threadIdx.x & 63, n16 = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int wr = wave / WC, wc = wave % WC;
+
+  // Tiles in bands of 4 rows of tiles, columns outer within a band; an XCD (b
+  // mod 8) takes consecutive ones, which share their panels in its L2.
+  const uint32_t tiles_all = static_cast<uint32_t>(p.row_tiles) * p.col_tiles;
+  const uint32_t per = (tiles_all + 7) / 8;
+  const uint32_t tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (tile >= tiles_all) return;
+  const uint32_t band = tile / (4u * p.col_tiles);
+  const uint32_t in_band = tile - band * 4u * p.col_tiles;
+  const uint32_t h = min(4u, static_cast<uint32_t>(p.row_tiles) - 4u * band);
+  const int ct = __builtin_amdgcn_readfirstlane(in_band / h);
+  const int rt = __builtin_amdgcn_readfirstlane(4 * band + in_band % h);
+  const int64_t xp0 = int64_t{rt} * XT, wp0 = int64_t{ct} * (SL / 2);
+  const int last_x = static_cast<int>(min(int64_t{XT}, p.x_panels - xp0)) - 1;
+  const int last_w = static_cast<int>(min(int64_t{SL / 2}, p.w_panels - wp0)) - 1;
+
+  // The wavefront's units. Panels past the last read the last one: their results
+  // are not stored. A unit's memory ends with its panel, so that what lies past k
+  // and past the last step reads as zeros.
+  const int steps = static_cast<int>(p.steps);
+  const uint32_t panel_bytes = static_cast<uint32_t>(p.k * kRows * sizeof(T));
+  Unit units[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) {
+    const int u = min(ND * wave + i, kUnits - 1);
+    units[i].at = static_cast<uint32_t>(u) * 1024u;
+    uint32_t first, bytes;
+    if (u < kXUnits) {
+      const int panel = u / XPL;
+      first = static_cast<uint32_t>(u % XPL) * 1024u;
+      bytes = static_cast<uint32_t>(steps) * (XPL * 1024u);
+      units[i].stride = XPL * 1024;
+      units[i].src = reinterpret_cast<const unsigned char*>(p.xp) +
+                     (xp0 + min(panel, last_x)) * static_cast<int64_t>(bytes) + first;
+    } else {
+      const int slot = (u - kXUnits) / WU;
+      first = static_cast<uint32_t>((u - kXUnits) % WU) * 1024u;
+      bytes = panel_bytes;
+      units[i].stride = WU * 1024;
+      units[i].src = static_cast<const unsigned char*>(p.wp[slot & 1]) +
+                     (wp0 + min(slot / 2, last_w)) * static_cast<int64_t>(bytes) + first;
+    }
+    units[i].size = bytes - min(bytes, first);
+  }
+  auto stage = [&](unsigned char* buf, int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+      LoadUnit(units[i], buf, static_cast<uint32_t>(t), lane);
+  };
+
+  f32x4_t acc[XP][WP];
+#pragma unroll
+  for (int a = 0; a < XP; ++a)
+#pragma unroll
+    for (int b = 0; b < WP; ++b) acc[a][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  auto compute = [&](const unsigned char* buf) __attribute__((always_inline)) {
+    s16x8_t x[XP][XPL];
+#pragma unroll
+    for (int a = 0; a < XP; ++a)
+#pragma unroll
+      for (int i = 0; i < XPL; ++i)
+        x[a][i] = *reinterpret_cast<const s16x8_t*>(buf + ((wr * XP + a) * XPL + i) * 1024 +
+                                                    lane * 16);
+#pragma unroll
+    for (int b = 0; b < WP; ++b) {
+      const unsigned char* const base = buf + (kXUnits + (wc * WP + b) * WU) * 1024;
+      s16x8_t w[WPL];
+      if constexpr (WT == EHIP_WEIGHT_F32) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          short parts[WPL];
+          Cut<WT>(reinterpret_cast<const float*>(base)[OperandK<WT>(q, e) * kRows + n16], parts);
+#pragma unroll
+          for (int j = 0; j < WPL; ++j) w[j][e] = parts[j];
+        }
+      } else {
+        const unsigned char* const at = base + ((4 * q + (n16 >> 2)) * kRows + 4 * (n16 & 3)) * 2;
+        w[0] = __builtin_shufflevector(TransposedRead(at), TransposedRead(at + 16 * kRows * 2), 0,
+                                       1, 2, 3, 4, 5, 6, 7);
+      }
+      // Products x_i w_j with i + j < planes of x, smallest first.
+#pragma unroll
+      for (int s = XPL - 1; s >= 0; --s)
+#pragma unroll
+        for (int j = 0; j < WPL; ++j)
+          if (s - j >= 0) {
+#pragma unroll
+            for (int a = 0; a < XP; ++a) acc[a][b] = Mfma<WT>(w[j], x[a][s - j], acc[a][b]);
+          }
+    }
+  };
+
+  // Step t waits for its own loads and meets the other wavefronts', then
+  // loads step t + NS - 1 into the buffer that step t - 1 has read. The loads stay
+  // unconditional (past the end: zeros), so that the count holds.
+  stage(b0, 0);
+  Fence();
+  if constexpr (NS > 2) stage(b1, 1);
+  Fence();
+  if constexpr (NS > 3) stage(b2, 2);
+  Fence();
+  int t = 0;
+  auto step = [&](auto s) __attribute__((always_inline)) {
+    constexpr int S = decltype(s)::value;
+    WaitAndMeet<(NS - 2) * ND>();
+    stage(Buffer<(S + NS - 1) % NS>(b0, b1, b2, b3), t + NS - 1);
+    Fence();
+    compute(Buffer<S % NS>(b0, b1, b2, b3));
+    return ++t >= steps;
+  };
+  for (;;) {
+    if (step(std::integral_constant<int, 0>{})) break;
+    if (step(std::integral_constant<int, 1>{})) break;
+    if (step(std::integral_constant<int, 2>{})) break;
+    if constexpr (NS != 3)
+      if (step(std::integral_constant<int, 3>{})) break;
+  }
+  // Loads past the end may still be in flight into the buffers: they land first.
+  constexpr int kFit = kFirst / kResults, PP = kFit >= 4 && XP % 4 == 0   ? 4
+                                                   : kFit >= 2 && XP % 2 == 0 ? 2
+                                                                              : 1;
+  WaitAndMeet<0>();
+  int down[XP];
+#pragma unroll
+  for (int a = 0; a < XP; ++a)
+    down[a] = WT == EHIP_WEIGHT_F16
+                  ? p.row_scale[(xp0 + min(wr * XP + a, last_x)) * kRows + n16]
+                  : 0;
+  StoreTile<XP, WP, PP, ACT, WT == EHIP_WEIGHT_F16>(
+      p, b0 + wave * (PP * C * 256), (xp0 + wr * XP) * kRows, (wp0 + wc * WP / 2) * kRows, acc,
+      down);
+}
+
+// Few rows (m <= MR): a workgroup per (panel, gate and up), its KW wavefronts
+// taking k in turn. A lane reads 16 bytes of a panel row (columns 8h.. of row k;
+// 4h.. in fp32) and multiplies them by x's MR values at that k, in fp32, into
+// sums of its own; the lanes of a column and the wavefronts meet in LDS, in
+// order. Bound by the panels' bytes up to eight rows.
+template <int WT, int MR, int KW, int ACT>
+__global__ __launch_bounds__(64 * KW) void GatedStream(GatedParams p) {
+  using T = typename Type<WT>::T;
+  constexpr int V = 16 / sizeof(T);        // columns of a lane
+  constexpr int L = kRows / V;             // lanes of a panel row
+  constexpr int KR = 64 / L;               // k rows of a wavefront's read
+  constexpr int U = 4;                     // reads in flight a projection
+  __shared__ float red[KW][2][MR][kRows];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int kr = lane / L, h = lane % L;
+  const int64_t panel = blockIdx.x;
+  const T* const w0 = static_cast<const T*>(p.wp[0]) + panel * p.k * kRows;
+  const T* const w1 = static_cast<const T*>(p.wp[1]) + panel * p.k * kRows;
+  float acc[2][MR][V];
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+#pragma unroll
+    for (int r = 0; r < MR; ++r)
+#pragma unroll
+      for (int c = 0; c < V; ++c) acc[g][r][c] = 0.f;
+  auto widen = [&](const i32x4_t& a, float (&v)[V]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u = static_cast<uint32_t>(a[i]);
+      if constexpr (WT == EHIP_WEIGHT_F32) {
+        v[i] = __uint_as_float(u);
+      } else if constexpr (WT == EHIP_WEIGHT_BF16) {
+        v[2 * i] = Bf16Lo(u);
+        v[2 * i + 1] = Bf16Hi(u);
+      } else {
+        v[2 * i] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(u)));
+        v[2 * i + 1] =
+            static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(u >> 16)));
+      }
+    }
+  };
+  for (int64_t k0 = int64_t{wave} * (KR * U); k0 < p.k; k0 += KW * KR * U) {
+    i32x4_t a[U][2];
+    float x[U][MR];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t kk = k0 + u * KR + kr;
+      const bool in = kk < p.k;
+      const int64_t at = (in ? kk : 0) * kRows + h * V;
+      a[u][0] = __builtin_nontemporal_load(reinterpret_cast<const i32x4_t*>(w0 + at));
+      a[u][1] = __builtin_nontemporal_load(reinterpret_cast<const i32x4_t*>(w1 + at));
+      if (!in) a[u][0] = a[u][1] = i32x4_t{0, 0, 0, 0};
+#pragma unroll
+      for (int r = 0; r < MR; ++r)
+        x[u][r] = in && r < p.m ? p.x[r * p.k + kk] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        float v[V];
+        widen(a[u][g], v);
+#pragma unroll
+        for (int r = 0; r < MR; ++r)
+#pragma unroll
+          for (int c = 0; c < V; ++c) acc[g][r][c] = __builtin_fmaf(x[u][r], v[c], acc[g][r][c]);
+      }
+  }
+  // Sum over the lanes of a column: those that differ above log2 L.
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+#pragma unroll
+    for (int r = 0; r < MR; ++r)
+#pragma unroll
+      for (int c = 0; c < V; ++c) {
+        float s = acc[g][r][c];
+        for (int d = L; d < 64; d *= 2) s += ShflXor(s, d);
+        if (kr == 0) red[wave][g][r][h * V + c] = s;
+      }
+  __syncthreads();
+  // Thread (row, column) of the panel's results.
+  for (int i = threadIdx.x; i < MR * kRows; i += 64 * KW) {
+    const int r = i / kRows, c = i % kRows;
+    const int64_t col = panel * kRows + c;
+    if (r >= p.m || col >= p.n) continue;
+    float g = red[0][0][r][c], u = red[0][1][r][c];
+    for (int w = 1; w < KW; ++w) {
+      g += red[w][0][r][c];
+      u += red[w][1][r][c];
+    }
+    if (p.bias[0]) g += p.bias[0][col];
+    if (p.bias[1]) u += p.bias[1][col];
+    p.y[r * p.n + col] = Activate<ACT>(g) * u;
+  }
+}
+
+// fp32 weights and up to some hundred rows: a workgroup per (XP panels of x, gate
+// and up panel), on the fp32 matrix-core product of 16 x 16 x 4, whose operands
+// need no cutting: a lane's weights are single words of a panel's rows, and its x
+// four consecutive k of one row, in which product i of four takes the i-th. The
+// wavefronts take 16 k in turn and meet in LDS, in order. Its products cost 2.7
+// times the planes', which the weights' bytes hide up to there.
+template <int XP, int KW, int ACT>
+__global__ __launch_bounds__(64 * KW) void GatedDirect(GatedParams p) {
+  __shared__ f32x4_t red[KW][XP * 2][64];
+  const int lane = threadIdx.x & 63, n16 = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const uint32_t xb = blockIdx.x / static_cast<uint32_t>(p.w_panels);
+  const int64_t wp = blockIdx.x - xb * static_cast<uint32_t>(p.w_panels);
+  const int64_t row0 = int64_t{xb} * XP * kRows + n16;
+  const float* const wg = static_cast<const float*>(p.wp[0]) + wp * p.k * kRows + n16;
+  const float* const wu = static_cast<const float*>(p.wp[1]) + wp * p.k * kRows + n16;
+  f32x4_t acc[XP][2];
+  const float* xr[XP];
+#pragma unroll
+  for (int a = 0; a < XP; ++a) {
+    acc[a][0] = acc[a][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    // Rows past the last read the last one: their results are not stored.
+    xr[a] = p.x + min(row0 + a * kRows, p.m - 1) * p.k;
+  }
+  f32x4_t x[XP], w[2];
+  auto load = [&](int64_t k0) __attribute__((always_inline)) {
+    const int64_t kk = k0 + 4 * q;
+    if (p.x_vec && k0 + 16 <= p.k) {
+#pragma unroll
+      for (int a = 0; a < XP; ++a) x[a] = *reinterpret_cast<const f32x4_t*>(xr[a] + kk);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[0][i] = wg[(kk + i) * kRows];
+        w[1][i] = wu[(kk + i) * kRows];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool in = kk + i < p.k;
+        const int64_t at = in ? kk + i : 0;
+#pragma unroll
+        for (int a = 0; a < XP; ++a) x[a][i] = in ? xr[a][at] : 0.f;
+        w[0][i] = in ? wg[at * kRows] : 0.f;
+        w[1][i] = in ? wu[at * kRows] : 0.f;
+      }
+    }
+  };
+  int64_t k0 = int64_t{wave} * 16;
+  if (k0 < p.k) load(k0);
+  for (; k0 < p.k; k0 += 16 * KW) {
+    f32x4_t cx[XP], cw[2] = {w[0], w[1]};
+#pragma unroll
+    for (int a = 0; a < XP; ++a) cx[a] = x[a];
+    if (k0 + 16 * KW < p.k) load(k0 + 16 * KW);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int a = 0; a < XP; ++a)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          acc[a][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(cw[h][i], cx[a][i], acc[a][h], 0, 0, 0);
+  }
+#pragma unroll
+  for (int a = 0; a < XP; ++a)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) red[wave][2 * a + h][lane] = acc[a][h];
+  __syncthreads();
+  for (int a = wave; a < XP; a += KW) {
+    f32x4_t s[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      s[h] = red[0][2 * a + h][lane];
+      for (int i = 1; i < KW; ++i) s[h] += red[i][2 * a + h][lane];
+    }
+    const int64_t col = wp * kRows + 4 * q;
+    StoreRow4<false>(p, row0 + a * kRows, col, Finish<ACT>(p, col, s[0], s[1]));
+  }
+}
+
+template <int XP, int ACT>
+hipError_t LaunchDirect(const GatedParams& p, hipStream_t stream) {
+  const int64_t n = (p.x_panels + XP - 1) / XP * p.w_panels;
+  if (n > INT32_MAX) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((GatedDirect<XP, 8, ACT>), dim3(static_cast<uint32_t>(n)), dim3(512), 0, stream,
+                     p);
+  return hipGetLastError();
+}
+
+template <int WT, int MR, int ACT>
+hipError_t LaunchStream(const GatedParams& p, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(p.w_panels));
+  hipLaunchKernelGGL((GatedStream<WT, MR, 8, ACT>), grid, dim3(512), 0, stream, p);
+  return hipGetLastError();
+}
+
+template <int WT, int WR, int WC, int XP, int WP, int NS, int ACT, int OCC>
+hipError_t LaunchTiles(GatedParams p, hipStream_t stream) {
+  const int64_t rt = (p.x_panels + WR * XP - 1) / (WR * XP);
+  const int64_t ct = (p.w_panels + WC * WP / 2 - 1) / (WC * WP / 2);
+  if (rt * ct > (int64_t{1} << 30)) return hipErrorInvalidValue;
+  p.row_tiles = static_cast<int32_t>(rt);
+  p.col_tiles = static_cast<int32_t>(ct);
+  const uint32_t grid = static_cast<uint32_t>((rt * ct + 7) / 8 * 8);
+  hipLaunchKernelGGL((GatedStaged<WT, WR, WC, XP, WP, NS, ACT, OCC>), dim3(grid),
+                     dim3(64 * WR * WC), 0, stream, p);
+  return hipGetLastError();
+}
+
+template <int WT>
+hipError_t LaunchCut(const GatedParams& p, hipStream_t stream) {
+  // A step a wavefront; for fp16, whose workgroups read all of their rows first,
+  // as many workgroups as two a CU.
+  int64_t chunks = (p.steps + 3) / 4;
+  if (WT == EHIP_WEIGHT_F16)
+    chunks = std::min(chunks, std::max<int64_t>(1, 512 / p.x_panels));
+  chunks = std::min<int64_t>(chunks, 65535);
+  const int chunk = static_cast<int>((p.steps + chunks - 1) / chunks);
+  const dim3 grid(static_cast<uint32_t>(p.x_panels),
+                  static_cast<uint32_t>((p.steps + chunk - 1) / chunk));
+  hipLaunchKernelGGL(CutRows<WT>, grid, dim3(256), 0, stream, p, chunk);
+  return hipGetLastError();
+}
+
+// The staged kernel's tile for a call, by an estimate of each one's time in us:
+// rounds of its workgroups over the chip (a part of one counts for 0.6 at least:
+// fewer workgroups on a CU run faster) times (steps times a step's time + the
+// time of filling and storing), for bf16 weights; fp16 ones take two thirds, in
+// all alike. Step times measured at 2382 x 4096 x 16384 and 64 x 4096 x 16384,
+// the rest at 2382 x 896 x 3584. What it picks (us, the tiles in the order below):
+// 2382 x 4096 x 16384 1313 of (1313, 1387, 1571, 1795), 600 rows 391 (391, 382,
+// 416, 471), 300 rows 222 (261, 236, 222, 267), 64 rows 70 (154, 110, 70, 82), 48
+// rows 59 (146, 97, 63, 59), 2382 x 896 x 3584 81 (94, 81, 81, 83).
+enum class Tile { k128x128, k128x64, k64x64, k48x32 };
+
+Tile PickTile(const GatedParams& p) {
+  struct Cost {
+    Tile tile;
+    int rows, cols;  // panels of x and of y
+    double step, fixed;
+  };
+  constexpr Cost kCosts[] = {{Tile::k128x128, 8, 8, 2.05, 25},
+                             {Tile::k128x64, 8, 4, 1.08, 7},
+                             {Tile::k64x64, 4, 4, 0.62, 2},
+                             {Tile::k48x32, 3, 2, 0.33, 2}};
+  Tile best = Tile::k128x128;
+  double least = 0;
+  for (const Cost& c : kCosts) {
+    const double tiles = static_cast<double>((p.x_panels + c.rows - 1) / c.rows) *
+                         static_cast<double>((p.w_panels + c.cols - 1) / c.cols);
+    const double us = std::max(0.6, tiles / 512) * (static_cast<double>(p.steps) * c.step + c.fixed);
+    if (least == 0 || us < least) {
+      least = us;
+      best = c.tile;
+    }
+  }
+  return best;
+}
+
+template <int WT, int ACT>
+hipError_t Launch(const GatedParams& p, hipStream_t stream) {
+  if (p.m <= 1) return LaunchStream<WT, 1, ACT>(p, stream);
+  if (p.m <= 2) return LaunchStream<WT, 2, ACT>(p, stream);
+  if (p.m <= 4) return LaunchStream<WT, 4, ACT>(p, stream);
+  if (p.m <= kStreamRows) return LaunchStream<WT, 8, ACT>(p, stream);
+  if constexpr (WT == EHIP_WEIGHT_F32) {
+    if (p.x_panels <= kDirectPanels) {
+      // As few groups of rows as there can be, alike.
+      const int64_t groups = (p.x_panels + 4) / 5;
+      switch ((p.x_panels + groups - 1) / groups) {
+        case 1: return LaunchDirect<1, ACT>(p, stream);
+        case 2: return LaunchDirect<2, ACT>(p, stream);
+        case 3: return LaunchDirect<3, ACT>(p, stream);
+        case 4: return LaunchDirect<4, ACT>(p, stream);
+        default: return LaunchDirect<5, ACT>(p, stream);
+      }
+    }
+    if (hipError_t e = LaunchCut<WT>(p, stream); e != hipSuccess) return e;
+    return LaunchTiles<WT, 1, 4, 8, 4, 2, ACT, 1>(p, stream);
+  } else {
+    if (hipError_t e = LaunchCut<WT>(p, stream); e != hipSuccess) return e;
+    constexpr bool kF16 = WT == EHIP_WEIGHT_F16;
+    switch (PickTile(p)) {
+      case Tile::k128x128: return LaunchTiles<WT, 1, 4, 8, 4, 2, ACT, 2>(p, stream);
+      case Tile::k128x64: return LaunchTiles<WT, 2, 2, 4, 4, kF16 ? 3 : 2, ACT, 2>(p, stream);
+      case Tile::k64x64: return LaunchTiles<WT, 2, 2, 2, 4, 4, ACT, 2>(p, stream);
+      default: return LaunchTiles<WT, 1, 4, 3, 2, 4, ACT, 2>(p, stream);
+    }
+  }
+}
+
+template <int WT>
+hipError_t LaunchType(const GatedParams& p, hipStream_t stream) {
+  switch (p.act) {
+    case EHIP_ACT_SILU: return Launch<WT, EHIP_ACT_SILU>(p, stream);
+    case EHIP_ACT_GELU: return Launch<WT, EHIP_ACT_GELU>(p, stream);
+    default: return Launch<WT, EHIP_ACT_GELU_TANH>(p, stream);
+  }
+}
+
+}  // namespace
+
+size_t PlanGatedGemm(int64_t m, int64_t k, int64_t n, int weight_dtype, GatedParams* p) {
+  p->m = m;
+  p->k = k;
+  p->n = n;
+  p->x_panels = (m + kRows - 1) / kRows;
+  p->w_panels = (n + kRows - 1) / kRows;
+  p->steps = (k + kStep - 1) / kStep;
+  if (m <= kStreamRows || (weight_dtype == EHIP_WEIGHT_F32 && p->x_panels <= kDirectPanels))
+    return 0;
+  const int planes = weight_dtype == EHIP_WEIGHT_F16 ? 2 : 3;
+  p->scale_at = static_cast<size_t>(p->x_panels) * static_cast<size_t>(p->steps) * planes * 1024;
+  return p->scale_at +
+         (weight_dtype == EHIP_WEIGHT_F16 ? static_cast<size_t>(p->x_panels) * kRows * 4 : 0);
+}
+
+hipError_t LaunchGatedGemm(const GatedParams& p, int weight_dtype, hipStream_t stream) {
+  switch (weight_dtype) {
+    case EHIP_WEIGHT_F32: return LaunchType<EHIP_WEIGHT_F32>(p, stream);
+    case EHIP_WEIGHT_BF16: return LaunchType<EHIP_WEIGHT_BF16>(p, stream);
+    case EHIP_WEIGHT_F16: return LaunchType<EHIP_WEIGHT_F16>(p, stream);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+}  // namespace ehip

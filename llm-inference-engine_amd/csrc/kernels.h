@@ -206,8 +206,8 @@ struct GemmParams {
   const void* wp;       // packed weight
   const float* bias;    // [n] or null
   float* y;             // [m, n]
-  float* part;          // partial sums (splits > 1): [splits, m, n] (gated: [splits, m, 2, n]),
-                        // or with tile_rows > 0 [split tiles, splits, tile_rows, 256]
+  float* part;          // partial sums (splits > 1): [splits, m, n], or with tile_rows > 0
+                        // [split tiles, splits, tile_rows, 256]
   int64_t m, k, n;
   int64_t m_pad, k_pad;  // m, k rounded up to whole 64 x 64 tiles
   int64_t panels;       // ceil(n / 16)
@@ -224,16 +224,9 @@ struct GemmParams {
   int32_t split_steps;
   int32_t items;        // workgroups
   int32_t slots;        // workgroups resident at once
-  // The gated block (projections = 2): y = act(x Wg^T + bias) * (x Wu^T + bias2),
-  // wp the gate's panels and wp2 the up projection's.
-  const void* wp2;
-  const float* bias2;
-  int32_t projections;
-  int32_t act;          // EHIP_ACT_*
 };
 // Tiles and k splits for a call (cus: the device's CU count).
-void PlanPackedGemm(int64_t m, int64_t k, int64_t n, int weight_dtype, int cus, GemmParams* p,
-                    bool gated = false);
+void PlanPackedGemm(int64_t m, int64_t k, int64_t n, int weight_dtype, int cus, GemmParams* p);
 // Workspace bytes of x's planes for the planned call.
 size_t PackedGemmPlaneBytes(const GemmParams& p);
 // Workspace bytes of the planned call's partial sums.
@@ -241,6 +234,26 @@ size_t PackedGemmPartBytes(const GemmParams& p);
 hipError_t LaunchPackedGemm(const GemmParams& p, int weight_dtype, hipStream_t stream);
 hipError_t LaunchPackWeightPanels(const void* w, int weight_dtype, int64_t n, int64_t k, void* wp,
                                   hipStream_t stream);
+
+// The gated feed-forward block (gated_gemm.hip): y[m, n] = act(x wp[0]^T +
+// bias[0]) * (x wp[1]^T + bias[1]) over packed weights.
+struct GatedParams {
+  const float* x;        // [m, k]
+  const void* wp[2];     // gate and up panels [w_panels, k, 16]
+  const float* bias[2];  // [n] or null
+  float* y;              // [m, n]
+  uint16_t* xp;          // x's planes in operand panels (workspace)
+  int32_t* row_scale;    // fp16: exponents of x's rows (workspace)
+  int64_t m, k, n;
+  int64_t x_panels, w_panels, steps;
+  size_t scale_at;       // bytes of the planes, where the row scales begin
+  int32_t x_vec, y_vec;  // rows are 16-byte aligned
+  int32_t act;           // EHIP_ACT_*
+  int32_t row_tiles, col_tiles;  // the staged kernel's (set at its launch)
+};
+// Sizes of a call; its workspace bytes.
+size_t PlanGatedGemm(int64_t m, int64_t k, int64_t n, int weight_dtype, GatedParams* p);
+hipError_t LaunchGatedGemm(const GatedParams& p, int weight_dtype, hipStream_t stream);
 
 // MXFP4 (mxfp4.hip; panel layout in mxfp4.h).
 inline int64_t MxPanels(int64_t rows) { return (rows + 15) / 16; }

@@ -50,26 +50,4 @@ __device__ __forceinline__ uint32_t MxCodes(const float (&v)[8], uint32_t byte) 
   return r;
 }
 
-// The feed-forward activations (EHIP_ACT_*), fp32. exp by the hardware's base-2
-// exponential (one unit in the last place) of x log2 e; 1 / (1 + exp) by its
-// reciprocal. An argument of -infinity gives NaN, as x / (1 + exp(-x)) does.
-template <int ACT>
-__device__ __forceinline__ float Activate(float x) {
-  if constexpr (ACT == EHIP_ACT_SILU) {
-    return x * __builtin_amdgcn_rcpf(1.f + Exp2(-kLog2e * x));
-  } else if constexpr (ACT == EHIP_ACT_GELU) {
-    return 0.5f * x * erfcf(-0.70710678118654752f * x);
-  } else {
-    // 0.5 (1 + tanh u) = 1 / (1 + exp(-2u)), u = sqrt(2 / pi) (x + 0.044715 x^3)
-    const float u = x * (1.f + 0.044715f * x * x);
-    return x * __builtin_amdgcn_rcpf(1.f + Exp2(-2.f * 0.79788456080286536f * kLog2e * u));
-  }
-}
-
-__device__ __forceinline__ float Activate(int act, float x) {
-  return act == EHIP_ACT_SILU   ? Activate<EHIP_ACT_SILU>(x)
-         : act == EHIP_ACT_GELU ? Activate<EHIP_ACT_GELU>(x)
-                                : Activate<EHIP_ACT_GELU_TANH>(x);
-}
-
 }  // namespace ehip

@@ -8,13 +8,12 @@
 
 #include "kernels.h"
 #include "mxfp4.h"
+#include "staged.h"
 
 namespace ehip {
 namespace {
 
 typedef __attribute__((ext_vector_type(8))) int i32x8_t;
-typedef __attribute__((ext_vector_type(4))) int i32x4_t;
-typedef __attribute__((ext_vector_type(4))) float f32x4_t;
 
 // ------------------------------------------------------------- quantisation --
 //
@@ -206,40 +205,6 @@ __device__ __forceinline__ f32x4_t MxMfma(const i32x4_t& w, uint32_t ws, const i
                                                           static_cast<int>(xs));
 }
 
-// ACT of a plain product; gated ones name their activation, so that a kernel
-// holds one activation's code (erfc alone is a hundred instructions a value).
-constexpr int kPlain = -1;
-
-// Biases, then the activation and the product, of four columns from `col`:
-// `up` the other projection's sums of a gated call.
-template <int ACT>
-__device__ __forceinline__ f32x4_t MxFinish(const MxGemmParams& p, int64_t col, f32x4_t g,
-                                            f32x4_t up) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const bool in = col + i < p.n;
-    float v = g[i] + (in && p.bias[0] ? p.bias[0][col + i] : 0.f);
-    if constexpr (ACT != kPlain)
-      v = Activate<ACT>(v) * (up[i] + (in && p.bias[1] ? p.bias[1][col + i] : 0.f));
-    g[i] = v;
-  }
-  return g;
-}
-
-// Four columns of a row of y, as far as they lie in it.
-__device__ __forceinline__ void MxStore(const MxGemmParams& p, int64_t row, int64_t col,
-                                        const f32x4_t& v) {
-  if (row >= p.m || col >= p.n) return;
-  float* y = p.y + row * p.n + col;
-  if (p.y_vec) {  // n % 4 == 0
-    __builtin_nontemporal_store(v, reinterpret_cast<f32x4_t*>(y));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (col + i < p.n) y[i] = v[i];
-  }
-}
-
 // Few rows: a workgroup per (MP x panels, one weight panel a projection), its KW
 // wavefronts taking the scale groups in turn with their operands straight from
 // memory into registers, a group ahead, then one sum over the wavefronts through
@@ -382,21 +347,8 @@ __global__ __launch_bounds__(64 * KW) void MxDirect(MxGemmParams p) {
       for (int i = 1; i < KW; ++i) s[h] += red[i][f * PR + h][lane];
     }
     const int64_t col = wp * kMxRows + 4 * block;
-    MxStore(p, (xp0 + f) * kMxRows + row, col, MxFinish<ACT>(p, col, s[0], s[PR - 1]));
+    StoreRow4<false>(p, (xp0 + f) * kMxRows + row, col, Finish<ACT>(p, col, s[0], s[PR - 1]));
   }
-}
-
-template <int I>
-__device__ __forceinline__ unsigned char* Buffer(unsigned char* b0, unsigned char* b1,
-                                                 unsigned char* b2, unsigned char* b3) {
-  return I == 0 ? b0 : I == 1 ? b1 : I == 2 ? b2 : b3;
-}
-
-// Waits until no more than N vector-memory operations and no LDS one of the
-// wavefront are outstanding, then for the other wavefronts.
-template <int N>
-__device__ __forceinline__ void WaitAndMeet() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
 // Many rows: a workgroup of WR x WC wavefronts per tile of WR XP x panels by WC WP
@@ -525,7 +477,6 @@ void MxStaged(MxGemmParams p) {
     for (int b = 0; b < WP; ++b) acc[a][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   uint32_t sx[XP], sw[WP], nx[XP], nw[WP];
 
-#define EHIP_MX_FENCE() asm volatile("" ::: "memory")
   auto turned = [&](const uint32_t (&ax)[XP], const uint32_t (&aw)[WP])
                     __attribute__((always_inline)) {
 #pragma unroll
@@ -534,16 +485,16 @@ void MxStaged(MxGemmParams p) {
     for (int b = 0; b < WP; ++b) sw[b] = __builtin_amdgcn_perm(0u, aw[b], bytes);
   };
   load_scales(0, nx, nw);
-  EHIP_MX_FENCE();
+  Fence();
   stage(b0, 0);
   if constexpr (WD > 0) load_w(wf[0], 0);
-  EHIP_MX_FENCE();
+  Fence();
   stage(b1, 1);
   if constexpr (WD > 2) load_w(wf[1], 1);
-  EHIP_MX_FENCE();
+  Fence();
   if constexpr (NS > 3) stage(b2, 2);
   if constexpr (WD > 2) load_w(wf[2], 2);
-  EHIP_MX_FENCE();
+  Fence();
   turned(nx, nw);
   auto compute = [&](auto j, const unsigned char* buf, i32x4_t (&w)[WP])
                      __attribute__((always_inline)) {
@@ -573,11 +524,11 @@ void MxStaged(MxGemmParams p) {
     WaitAndMeet<kPending>();
     if constexpr (J == 0) {
       load_scales(g + 1, nx, nw);
-      EHIP_MX_FENCE();
+      Fence();
     }
     stage(Buffer<(S + NS - 1) % NS>(b0, b1, b2, b3), 4 * g + J + NS - 1);
     if constexpr (WD > 0) load_w(wf[(S + WD - 1) % kW], 4 * g + J + WD - 1);
-    EHIP_MX_FENCE();
+    Fence();
     compute(std::integral_constant<int, J>{}, Buffer<S % NS>(b0, b1, b2, b3),
             wf[S % kW]);
     return 4 * g + J + 1 >= p.tiles;
@@ -599,38 +550,14 @@ void MxStaged(MxGemmParams p) {
       if (group(std::integral_constant<int, 8>{})) break;
     }
   }
-#undef EHIP_MX_FENCE
 
-  // Results through LDS, so that a store instruction writes whole runs of a
-  // wavefront's columns (256 bytes a row; gated 128) instead of 64-byte pieces of
-  // 16 rows. Loads past the end may still be in flight into the buffers: they
-  // land first. A wavefront's part: PP panels' rows, 16-byte chunk c of row r at
-  // c ^ r (16 lanes of a pass hit distinct banks).
-  constexpr int kFit = kFirst / kResults;
-  constexpr int PP = kFit >= 4 ? 4 : kFit >= 2 ? 2 : 1;
-  static_assert(kFit >= 1 && XP % PP == 0 && (C & (C - 1)) == 0, "whole passes");
-  unsigned char* const part = b0 + wave * (PP * C * 256);
+  // Loads past the end may still be in flight into the buffers: they land first.
+  constexpr int kFit = kFirst / kResults, PP = kFit >= 4 ? 4 : kFit >= 2 ? 2 : 1;
   WaitAndMeet<0>();
-  const int64_t col0 = (wp0 + (GATED ? wc * WP / 2 : wc * WP)) * kMxRows;
-  const int n16 = lane & 15, q = lane >> 4;
-#pragma unroll
-  for (int a0 = 0; a0 < XP; a0 += PP) {
-#pragma unroll
-    for (int a = 0; a < PP; ++a)
-#pragma unroll
-      for (int b = 0; b < WP; b += GATED ? 2 : 1) {
-        const int c = (GATED ? b / 2 : b) * 4 + q;
-        *reinterpret_cast<f32x4_t*>(part + ((a * 16 + n16) * C + ((c ^ n16) & (C - 1))) * 16) =
-            MxFinish<ACT>(p, col0 + 4 * c, acc[a0 + a][b], acc[a0 + a][GATED ? b + 1 : b]);
-      }
-#pragma unroll
-    for (int i = 0; i < PP * 16 * C / 64; ++i) {
-      const int r = i * (64 / C) + lane / C, c = lane % C;
-      const f32x4_t v =
-          *reinterpret_cast<const f32x4_t*>(part + (r * C + ((c ^ r) & (C - 1))) * 16);
-      MxStore(p, (xp0 + wr * XP + a0) * kMxRows + r, col0 + 4 * c, v);
-    }
-  }
+  const int unscaled[XP] = {};
+  StoreTile<XP, WP, PP, ACT, false>(p, b0 + wave * (PP * C * 256), (xp0 + wr * XP) * kMxRows,
+                                    (wp0 + (GATED ? wc * WP / 2 : wc * WP)) * kMxRows, acc,
+                                    unscaled);
 }
 
 template <int WR, int WC, int XP, int WP, int NS, int WD, int ACT, int OCC>

@@ -43,7 +43,6 @@
 #include <cstdint>
 
 #include "kernels.h"
-#include "mxfp4.h"
 
 namespace ehip {
 namespace {
@@ -111,9 +110,7 @@ __device__ __forceinline__ bf16x4_t TransposedRead(const __bf16* p) {
   return __builtin_bit_cast(bf16x4_t, r);
 }
 
-// GATED: panel slots are pairs, gate panel j and up panel j (p.wp2), so that a
-// wavefront's neighbouring blocks are the two projections of the same columns.
-template <int WT, int BP, bool GATED>
+template <int WT, int BP>
 __global__ __launch_bounds__(kThreads) void PackedGemmMfma(GemmParams p) {
   using W = WeightType<WT>;
   using T = typename W::T;
@@ -135,7 +132,7 @@ __global__ __launch_bounds__(kThreads) void PackedGemmMfma(GemmParams p) {
   const int wr = wave >> 1;  // rows 32*wr .. +32 of the tile
   const int wc = wave & 1;   // panels NW*wc .. +NW of the tile
   const int64_t m0 = int64_t{blockIdx.y} * kBM;
-  const int pb = static_cast<int>(blockIdx.x) * (GATED ? kBP / 2 : kBP);
+  const int pb = static_cast<int>(blockIdx.x) * kBP;
   const int split = blockIdx.z;
   const int64_t kb = int64_t{split} * p.k_split;
   const int64_t ke = kb + p.k_split < p.k ? kb + p.k_split : p.k;
@@ -155,10 +152,8 @@ __global__ __launch_bounds__(kThreads) void PackedGemmMfma(GemmParams p) {
   const int64_t plane = p.m_pad * p.k_pad;
   const __bf16* xrow = reinterpret_cast<const __bf16*>(p.xp) + (m0 + xr) * p.k_pad;
   const int wpp = tid / KS, wk = tid % KS;  // panel wpp, k rows wk + KS * h
-  const int w_panel = pb + (GATED ? wpp >> 1 : wpp);
-  const bool w_ok = w_panel < p.panels;
-  const T* wpanel = static_cast<const T*>(GATED && (wpp & 1) ? p.wp2 : p.wp) +
-                    (w_ok ? int64_t{w_panel} * p.k * kNr : 0);
+  const bool w_ok = pb + wpp < p.panels;
+  const T* wpanel = static_cast<const T*>(p.wp) + (w_ok ? int64_t{pb + wpp} * p.k * kNr : 0);
 
   bf16x8_t xv[kXP][2];
   uint4 wv[RPT][WE];
@@ -273,31 +268,6 @@ __global__ __launch_bounds__(kThreads) void PackedGemmMfma(GemmParams p) {
     compute();
   }
 
-  if constexpr (GATED) {
-#pragma unroll
-    for (int cb = 0; cb < NW; cb += 2) {
-      const int64_t col = int64_t{pb + (NW * wc + cb) / 2} * kNr + n16;
-      if (col >= p.n) continue;
-      const float bg = (p.splits == 1 && p.bias) ? p.bias[col] : 0.f;
-      const float bu = (p.splits == 1 && p.bias2) ? p.bias2[col] : 0.f;
-#pragma unroll
-      for (int rb = 0; rb < 2; ++rb)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int64_t row = m0 + 32 * wr + 16 * rb + 4 * q + i;
-          if (row >= p.m) continue;
-          if (p.splits == 1) {
-            p.y[row * p.n + col] =
-                Activate(p.act, acc[rb][cb][i] + bg) * (acc[rb][cb + 1][i] + bu);
-          } else {
-            float* const part = p.part + (int64_t{split} * p.m + row) * 2 * p.n + col;
-            part[0] = acc[rb][cb][i];
-            part[p.n] = acc[rb][cb + 1][i];
-          }
-        }
-    }
-    return;
-  }
   // acc[rb][cb][i] = y[row 32wr + 16rb + 4q + i][column of panel NW wc + cb, n16].
 #pragma unroll
   for (int cb = 0; cb < NW; ++cb) {
@@ -356,7 +326,7 @@ struct WideShape {
   static constexpr int CB = kWideN / (8 / WR) / 16;            // panels per wavefront
 };
 
-template <int TM, int OCC, bool GATED>
+template <int TM, int OCC>
 __global__ __launch_bounds__(kWideThreads) __attribute__((amdgpu_waves_per_eu(OCC)))
 void PackedGemmWide(GemmParams p) {
   using S = WideShape<TM>;
@@ -400,7 +370,7 @@ void PackedGemmWide(GemmParams p) {
   const int ct = __builtin_amdgcn_readfirstlane(in_band / h);
   const int rt = __builtin_amdgcn_readfirstlane(4 * band + in_band - ct * h);
   const int64_t m0 = int64_t{rt} * TM;
-  const int pb = ct * (GATED ? 8 : 16);
+  const int pb = ct * 16;
   const int steps_all = static_cast<int>(p.k / kWideK);
   const int s0 = __builtin_amdgcn_readfirstlane(nsplit > 1 ? split * p.split_steps : 0);
   const int steps = nsplit > 1 ? min(p.split_steps, steps_all - s0) : steps_all;
@@ -411,17 +381,12 @@ void PackedGemmWide(GemmParams p) {
   const int64_t row_in = min(int64_t{xr}, p.m - 1 - m0);
   const uint32_t xoff = static_cast<uint32_t>(row_in * p.k * 4) + (tid & 3) * 16;
   const uint32_t pan0 = static_cast<uint32_t>(min(int64_t{wave}, p.panels - 1 - pb));
-  const uint32_t pan1 =
-      GATED ? pan0 : static_cast<uint32_t>(min(int64_t{wave + 8}, p.panels - 1 - pb));
+  const uint32_t pan1 = static_cast<uint32_t>(min(int64_t{wave + 8}, p.panels - 1 - pb));
   const uint32_t panel_b = static_cast<uint32_t>(p.k * kNr * 2);
   const uint32_t woff0 = pan0 * panel_b + lane * 16;
   const uint32_t woff1 = pan1 * panel_b + lane * 16;
   const float* const xbase = p.x + m0 * p.k;
   const uint16_t* const wbase = static_cast<const uint16_t*>(p.wp) + int64_t{pb} * p.k * kNr;
-  // GATED: gate panel j and up panel j are the tile's panels 2j and 2j + 1.
-  const uint16_t* const wbase2 =
-      GATED ? static_cast<const uint16_t*>(p.wp2) + int64_t{pb} * p.k * kNr : wbase;
-  const int slot0 = GATED ? 2 * wave : wave, slot1 = GATED ? slot0 + 1 : wave + 8;
   struct Stage {
     u32x4_t x[2];
     u32x4_t w[2];
@@ -433,15 +398,12 @@ void PackedGemmWide(GemmParams p) {
         __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(xbase), 0, size, 0x00020000);
     const __amdgpu_buffer_rsrc_t rw =
         __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(wbase), 0, size, 0x00020000);
-    const __amdgpu_buffer_rsrc_t rw2 =
-        GATED ? __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(wbase2), 0, size, 0x00020000)
-              : rw;
     const uint32_t xk = static_cast<uint32_t>(s0 + t) * (kWideK * 4);
     const uint32_t wk = static_cast<uint32_t>(s0 + t) * (kWideK * kNr * 2);
     st.x[0] = __builtin_amdgcn_raw_buffer_load_b128(rx, xoff, xk, 0);
     st.x[1] = __builtin_amdgcn_raw_buffer_load_b128(rx, xoff + 64, xk, 0);
     st.w[0] = __builtin_amdgcn_raw_buffer_load_b128(rw, woff0, wk, 0);
-    st.w[1] = __builtin_amdgcn_raw_buffer_load_b128(rw2, woff1, wk, 0);
+    st.w[1] = __builtin_amdgcn_raw_buffer_load_b128(rw, woff1, wk, 0);
   };
   auto store = [&](const Stage& st, int buf) __attribute__((always_inline)) {
     uint32_t pl[4][kXP];
@@ -464,8 +426,8 @@ void PackedGemmWide(GemmParams p) {
     for (int a = 0; a < kXP; ++a)
       *reinterpret_cast<u32x4_t*>(&xs[buf][a][xr * kWideK + (tid & 3) * 8]) =
           u32x4_t{pl[0][a], pl[1][a], pl[2][a], pl[3][a]};
-    *reinterpret_cast<u32x4_t*>(&ws[buf][slot0 * 512 + lane * 8]) = st.w[0];
-    *reinterpret_cast<u32x4_t*>(&ws[buf][slot1 * 512 + lane * 8]) = st.w[1];
+    *reinterpret_cast<u32x4_t*>(&ws[buf][wave * 512 + lane * 8]) = st.w[0];
+    *reinterpret_cast<u32x4_t*>(&ws[buf][(wave + 8) * 512 + lane * 8]) = st.w[1];
   };
 
   f32x4_t acc[RB][CB];
@@ -535,24 +497,6 @@ void PackedGemmWide(GemmParams p) {
       }
     return;
   }
-  if constexpr (GATED) {
-#pragma unroll
-    for (int cb = 0; cb < CB; cb += 2) {
-      const int64_t col = int64_t{pb + (CB * wc + cb) / 2} * kNr + n16;
-      if (col >= p.n) continue;
-      const float bg = p.bias ? p.bias[col] : 0.f, bu = p.bias2 ? p.bias2[col] : 0.f;
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int64_t row = m0 + 16 * (RB * wr + rb) + 4 * q + i;
-          if (row < p.m)
-            p.y[row * p.n + col] =
-                Activate(p.act, acc[rb][cb][i] + bg) * (acc[rb][cb + 1][i] + bu);
-        }
-    }
-    return;
-  }
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb) {
     const int64_t col = int64_t{pb + CB * wc + cb} * kNr + n16;
@@ -600,38 +544,6 @@ __global__ __launch_bounds__(256) void WideSplitReduce(GemmParams p, int tm) {
     if (col + i < p.n) p.y[r * p.n + col + i] = p.bias ? v[i] + p.bias[col + i] : v[i];
 }
 
-// The gated split tiles: both projections' partials in split order, biases,
-// then the activation and the product; a tile's 256 columns are 128 of y.
-__global__ __launch_bounds__(256) void WideSplitReduceGated(GemmParams p, int tm) {
-  const int quads = tm * (kWideN / 8);
-  const int e = static_cast<int>(blockIdx.y) * 256 + threadIdx.x;
-  if (e >= quads) return;
-  const int rt = static_cast<int>(blockIdx.x);
-  const int tile = rt + p.full_tiles;
-  const int band = tile / (4 * p.col_tiles);
-  const int in_band = tile - band * 4 * p.col_tiles;
-  const int h = min(4, p.row_tiles - 4 * band);
-  const int ct = in_band / h;
-  const int row = e / (kWideN / 8), c = (e - row * (kWideN / 8)) * 4;
-  const int64_t r = int64_t{4 * band + in_band - ct * h} * tm + row;
-  const int64_t col = int64_t{ct} * (kWideN / 2) + c;
-  if (r >= p.m || col >= p.n) return;
-  const int64_t size = int64_t{tm} * kWideN;
-  const float* part = p.part + int64_t{rt} * p.splits * size + row * kWideN +
-                      (c / kNr) * 2 * kNr + c % kNr;
-  f32x4_t g = *reinterpret_cast<const f32x4_t*>(part);
-  f32x4_t u = *reinterpret_cast<const f32x4_t*>(part + kNr);
-  for (int i = 1; i < p.splits; ++i) {
-    g += *reinterpret_cast<const f32x4_t*>(part + i * size);
-    u += *reinterpret_cast<const f32x4_t*>(part + i * size + kNr);
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (col + i < p.n)
-      p.y[r * p.n + col + i] = Activate(p.act, p.bias ? g[i] + p.bias[col + i] : g[i]) *
-                               (p.bias2 ? u[i] + p.bias2[col + i] : u[i]);
-}
-
 // x [m, k] fp32 -> its three bf16 planes [3][m_pad][k_pad], zero past m and
 // k; one thread per 8 consecutive elements of a padded row.
 __global__ __launch_bounds__(256) void SplitRows(GemmParams p, __bf16* xp) {
@@ -673,23 +585,6 @@ __global__ __launch_bounds__(256) void GemmSplitReduce(GemmParams p) {
   for (int sp = 1; sp < p.splits; ++sp) s += p.part[int64_t{sp} * total + i];
   if (p.bias) s += p.bias[i % p.n];
   p.y[i] = s;
-}
-
-// The gated form: partials [splits][m][2][n].
-__global__ __launch_bounds__(256) void GemmSplitReduceGated(GemmParams p) {
-  const int64_t total = p.m * p.n;
-  const int64_t i = int64_t{blockIdx.x} * 256 + threadIdx.x;
-  if (i >= total) return;
-  const int64_t row = i / p.n, col = i - row * p.n;
-  const float* part = p.part + row * 2 * p.n + col;
-  float g = part[0], u = part[p.n];
-  for (int sp = 1; sp < p.splits; ++sp) {
-    g += part[int64_t{sp} * 2 * total];
-    u += part[int64_t{sp} * 2 * total + p.n];
-  }
-  if (p.bias) g += p.bias[col];
-  if (p.bias2) u += p.bias2[col];
-  p.y[i] = Activate(p.act, g) * u;
 }
 
 // Wp[p, kk, r] = W[p*16 + r, kk] (0 past n): the reference's PackWeightPanels
@@ -737,7 +632,7 @@ bool PlanWide(int64_t m, int64_t k, int64_t n, int cus, GemmParams* p) {
   // other one has 256-column tiles, 14.5/12.8 at k = 64 and 200 rows.
   if (k < 256 && m > 256) return false;
   const int tm = WideRows(m);
-  const int64_t rt = (m + tm - 1) / tm, ct = (p->panels * p->projections + 15) / 16;
+  const int64_t rt = (m + tm - 1) / tm, ct = (p->panels + 15) / 16;
   if (rt * ct > (int64_t{1} << 24)) return false;
   const int steps = static_cast<int>(k / kWideK);
   p->tile_rows = tm;
@@ -767,9 +662,7 @@ bool PlanWide(int64_t m, int64_t k, int64_t n, int cus, GemmParams* p) {
 
 }  // namespace
 
-void PlanPackedGemm(int64_t m, int64_t k, int64_t n, int weight_dtype, int cus, GemmParams* p,
-                    bool gated) {
-  p->projections = gated ? 2 : 1;
+void PlanPackedGemm(int64_t m, int64_t k, int64_t n, int weight_dtype, int cus, GemmParams* p) {
   p->m = m;
   p->k = k;
   p->n = n;
@@ -785,7 +678,7 @@ void PlanPackedGemm(int64_t m, int64_t k, int64_t n, int weight_dtype, int cus, 
   p->group_panels = kBP;
   p->m_pad = (m + kBM - 1) / kBM * kBM;
   p->k_pad = (k + kBK - 1) / kBK * kBK;
-  const int64_t tiles = ((m + kBM - 1) / kBM) * ((p->panels * p->projections + kBP - 1) / kBP);
+  const int64_t tiles = ((m + kBM - 1) / kBM) * ((p->panels + kBP - 1) / kBP);
   const int64_t steps = (k + kBK - 1) / kBK;
   // Enough workgroups for one round at the tile's occupancy (two per CU for
   // the 256-column tile, about four otherwise: a workgroup keeps one step of
@@ -807,7 +700,7 @@ size_t PackedGemmPartBytes(const GemmParams& p) {
   if (p.tile_rows > 0)
     return static_cast<size_t>(p.items - p.full_tiles) * p.tile_rows * kWideN * sizeof(float);
   return static_cast<size_t>(p.splits) * static_cast<size_t>(p.m) * static_cast<size_t>(p.n) *
-         static_cast<size_t>(p.projections) * sizeof(float);
+         sizeof(float);
 }
 
 size_t PackedGemmPlaneBytes(const GemmParams& p) {
@@ -816,85 +709,62 @@ size_t PackedGemmPlaneBytes(const GemmParams& p) {
          sizeof(uint16_t);
 }
 
-namespace {
-
-template <bool GATED>
-hipError_t LaunchWide(const GemmParams& p, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(p.items)), block(kWideThreads);
-  switch (p.tile_rows) {
-    case 128:
-      hipLaunchKernelGGL((PackedGemmWide<128, 2, GATED>), grid, block, 0, stream, p);
-      break;
-    case 64:
-      hipLaunchKernelGGL((PackedGemmWide<64, 2, GATED>), grid, block, 0, stream, p);
-      break;
-    case 32:
-      hipLaunchKernelGGL((PackedGemmWide<32, 4, GATED>), grid, block, 0, stream, p);
-      break;
-    default:
-      hipLaunchKernelGGL((PackedGemmWide<16, 4, GATED>), grid, block, 0, stream, p);
-      break;
+hipError_t LaunchPackedGemm(const GemmParams& p, int weight_dtype, hipStream_t stream) {
+  if (p.tile_rows > 0) {
+    const dim3 grid(static_cast<uint32_t>(p.items)), block(kWideThreads);
+    switch (p.tile_rows) {
+      case 128:
+        hipLaunchKernelGGL((PackedGemmWide<128, 2>), grid, block, 0, stream, p);
+        break;
+      case 64:
+        hipLaunchKernelGGL((PackedGemmWide<64, 2>), grid, block, 0, stream, p);
+        break;
+      case 32:
+        hipLaunchKernelGGL((PackedGemmWide<32, 4>), grid, block, 0, stream, p);
+        break;
+      default:
+        hipLaunchKernelGGL((PackedGemmWide<16, 4>), grid, block, 0, stream, p);
+        break;
+    }
+    if (hipError_t e = hipGetLastError(); e != hipSuccess || p.splits == 1) return e;
+    const int tiles = (p.items - p.full_tiles) / p.splits;
+    hipLaunchKernelGGL(WideSplitReduce,
+                       dim3(static_cast<uint32_t>(tiles),
+                            static_cast<uint32_t>((p.tile_rows * (kWideN / 4) + 255) / 256)),
+                       dim3(256), 0, stream, p, static_cast<int>(p.tile_rows));
+    return hipGetLastError();
   }
-  if (hipError_t e = hipGetLastError(); e != hipSuccess || p.splits == 1) return e;
-  const uint32_t tiles = static_cast<uint32_t>((p.items - p.full_tiles) / p.splits);
-  const int quads = p.tile_rows * (GATED ? kWideN / 8 : kWideN / 4);
-  const dim3 reduce(tiles, static_cast<uint32_t>((quads + 255) / 256));
-  if constexpr (GATED)
-    hipLaunchKernelGGL(WideSplitReduceGated, reduce, dim3(256), 0, stream, p,
-                       static_cast<int>(p.tile_rows));
-  else
-    hipLaunchKernelGGL(WideSplitReduce, reduce, dim3(256), 0, stream, p,
-                       static_cast<int>(p.tile_rows));
-  return hipGetLastError();
-}
-
-template <bool GATED>
-hipError_t LaunchPlanes(const GemmParams& p, int weight_dtype, hipStream_t stream) {
   {
     const int64_t groups = p.m_pad * (p.k_pad / 8);
     hipLaunchKernelGGL(SplitRows, dim3(static_cast<uint32_t>((groups + 255) / 256)), dim3(256), 0,
                        stream, p, reinterpret_cast<__bf16*>(p.xp));
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
-  const dim3 grid(
-      static_cast<uint32_t>((p.panels * p.projections + p.group_panels - 1) / p.group_panels),
-      static_cast<uint32_t>((p.m + kBM - 1) / kBM), static_cast<uint32_t>(p.splits));
-  const dim3 block(kThreads);
+  const dim3 grid(static_cast<uint32_t>((p.panels + p.group_panels - 1) / p.group_panels),
+                  static_cast<uint32_t>((p.m + kBM - 1) / kBM), static_cast<uint32_t>(p.splits));
   switch (weight_dtype) {
     case EHIP_WEIGHT_F32:
-      hipLaunchKernelGGL((PackedGemmMfma<EHIP_WEIGHT_F32, 8, GATED>), grid, block, 0, stream, p);
+      hipLaunchKernelGGL((PackedGemmMfma<EHIP_WEIGHT_F32, 8>), grid, dim3(kThreads), 0, stream, p);
       break;
     case EHIP_WEIGHT_BF16:
       if (p.group_panels == 16)
-        hipLaunchKernelGGL((PackedGemmMfma<EHIP_WEIGHT_BF16, 16, GATED>), grid, block, 0, stream,
+        hipLaunchKernelGGL((PackedGemmMfma<EHIP_WEIGHT_BF16, 16>), grid, dim3(kThreads), 0, stream,
                            p);
       else
-        hipLaunchKernelGGL((PackedGemmMfma<EHIP_WEIGHT_BF16, 8, GATED>), grid, block, 0, stream,
+        hipLaunchKernelGGL((PackedGemmMfma<EHIP_WEIGHT_BF16, 8>), grid, dim3(kThreads), 0, stream,
                            p);
       break;
     case EHIP_WEIGHT_F16:
-      hipLaunchKernelGGL((PackedGemmMfma<EHIP_WEIGHT_F16, 8, GATED>), grid, block, 0, stream, p);
+      hipLaunchKernelGGL((PackedGemmMfma<EHIP_WEIGHT_F16, 8>), grid, dim3(kThreads), 0, stream, p);
       break;
     default:
       return hipErrorInvalidValue;
   }
   if (hipError_t e = hipGetLastError(); e != hipSuccess || p.splits == 1) return e;
   const int64_t total = p.m * p.n;
-  const dim3 reduce(static_cast<uint32_t>((total + 255) / 256));
-  if constexpr (GATED)
-    hipLaunchKernelGGL(GemmSplitReduceGated, reduce, dim3(256), 0, stream, p);
-  else
-    hipLaunchKernelGGL(GemmSplitReduce, reduce, dim3(256), 0, stream, p);
+  hipLaunchKernelGGL(GemmSplitReduce, dim3(static_cast<uint32_t>((total + 255) / 256)), dim3(256),
+                     0, stream, p);
   return hipGetLastError();
-}
-
-}  // namespace
-
-hipError_t LaunchPackedGemm(const GemmParams& p, int weight_dtype, hipStream_t stream) {
-  if (p.tile_rows > 0)
-    return p.projections == 2 ? LaunchWide<true>(p, stream) : LaunchWide<false>(p, stream);
-  return p.projections == 2 ? LaunchPlanes<true>(p, weight_dtype, stream)
-                            : LaunchPlanes<false>(p, weight_dtype, stream);
 }
 
 hipError_t LaunchPackWeightPanels(const void* w, int weight_dtype, int64_t n, int64_t k, void* wp,
