@@ -1013,6 +1013,7 @@ int ehip_packed_gated_gemm(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k
     return SetError(ctx, EHIP_INVALID_ARGUMENT,
                     "gated gemm: the packed weights must be 16-byte aligned (ehip_malloc gives 256)");
   ehip::GatedParams p{};
+  p.cus = ctx->cus;
   if (int rc = EnsureGemmWorkspace(ctx, ehip::PlanGatedGemm(m, k, n, weight_dtype, &p))) return rc;
   p.x = d_x;
   p.wp[0] = d_wp_gate;

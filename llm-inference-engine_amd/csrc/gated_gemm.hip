@@ -31,7 +31,7 @@ typedef __attribute__((ext_vector_type(4))) short s16x4_t;
 typedef __attribute__((ext_vector_type(8))) short s16x8_t;
 
 constexpr int kStreamRows = 8;     // up to these: GatedStream
-constexpr int kDirectPanels = 16;  // up to these, fp32 weights: GatedDirect
+constexpr int kDirectPanels = 8;   // up to these, fp32 weights: GatedDirect
 
 constexpr int kRows = 16;   // rows of a panel, of x or a weight
 constexpr int kStep = 32;   // k of a step
@@ -79,55 +79,61 @@ __device__ __forceinline__ void Cut(float v, short (&out)[Type<WT>::XPL]) {
   }
 }
 
+// The lane exchange CTRL (device_util.h) of an integer.
+template <int CTRL>
+__device__ __forceinline__ uint32_t Moved(uint32_t v) {
+  return static_cast<uint32_t>(
+      __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, false));
+}
+
 // x [m, k] into operand panels [panels][steps][planes][64 lanes][8]: zero past m
 // and k. A workgroup takes a panel's steps [chunk * blockIdx.y, ..), a wavefront a
 // step at a time; for fp16 every workgroup of a panel first finds its rows'
 // largest magnitudes.
-template <int WT>
-__global__ __launch_bounds__(256) void CutRows(GatedParams p, int chunk) {
+template <int WT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void CutRows(GatedParams p, int chunk) {
   constexpr int PL = Type<WT>::XPL;
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   const int64_t panel = blockIdx.x, row = panel * kRows + r;
   const float* const src = p.x + (row < p.m ? row : 0) * p.k;
   int up = 0;
   if constexpr (WT == EHIP_WEIGHT_F16) {
-    // 16 threads a row. As integers: the order of non-negative floats, NaN and
+    // A wavefront a row. As integers: the order of non-negative floats, NaN and
     // infinities on top (such a row is left as it is).
+    static_assert(WT != EHIP_WEIGHT_F16 || WAVES == kRows, "a wavefront a row");
     __shared__ int scale[kRows];
-    const int mine = threadIdx.x >> 4, i = threadIdx.x & 15;
+    const int mine = threadIdx.x >> 6;
     const int64_t at = panel * kRows + mine;
     uint32_t top = 0;
     if (at < p.m) {
       const float* const from = p.x + at * p.k;
-      int64_t kk = 0;
       if (p.x_vec) {
 #pragma unroll 4
-        for (kk = 4 * i; kk + 4 <= p.k; kk += 64) {
+        for (int64_t kk = 4 * lane; kk < p.k; kk += 256) {
           const f32x4_t a = *reinterpret_cast<const f32x4_t*>(from + kk);
 #pragma unroll
           for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(a[e]) & 0x7FFFFFFFu);
         }
       } else {
 #pragma unroll 4
-        for (kk = i; kk < p.k; kk += 16) top = max(top, __float_as_uint(from[kk]) & 0x7FFFFFFFu);
+        for (int64_t kk = lane; kk < p.k; kk += 64)
+          top = max(top, __float_as_uint(from[kk]) & 0x7FFFFFFFu);
       }
     }
-    top = max(top, static_cast<uint32_t>(
-                       __builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0xB1, 0xF, 0xF, false)));
-    top = max(top, static_cast<uint32_t>(
-                       __builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0x4E, 0xF, 0xF, false)));
-    top = max(top, static_cast<uint32_t>(
-                       __builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0x141, 0xF, 0xF, false)));
-    top = max(top, static_cast<uint32_t>(
-                       __builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0x128, 0xF, 0xF, false)));
+    top = max(top, Moved<0xB1>(top));
+    top = max(top, Moved<0x4E>(top));
+    top = max(top, Moved<0x141>(top));
+    top = max(top, Moved<0x128>(top));
+    top = max(top, __float_as_uint(ShflXor(__uint_as_float(top), 16)));
+    top = max(top, __float_as_uint(ShflXor(__uint_as_float(top), 32)));
     const int f = static_cast<int>(top >> 23);
-    if (i == 0) scale[mine] = f == 255 ? 0 : 14 + 127 - f;
+    if (lane == 0) scale[mine] = f == 255 ? 0 : 14 + 127 - f;
     __syncthreads();
     up = scale[r];
     if (blockIdx.y == 0 && threadIdx.x < kRows) p.row_scale[row] = -up;
   }
   const int64_t s0 = int64_t{blockIdx.y} * chunk, s1 = min(s0 + chunk, p.steps);
-  for (int64_t s = s0 + (threadIdx.x >> 6); s < s1; s += 4) {
+  for (int64_t s = s0 + (threadIdx.x >> 6); s < s1; s += WAVES) {
     float v[8];
     if constexpr (WT == EHIP_WEIGHT_F32) {
 #pragma unroll
@@ -357,15 +363,16 @@ void GatedStaged(GatedParams p) {
 // Few rows (m <= MR): a workgroup per (panel, gate and up), its KW wavefronts
 // taking k in turn. A lane reads 16 bytes of a panel row (columns 8h.. of row k;
 // 4h.. in fp32) and multiplies them by x's MR values at that k, in fp32, into
-// sums of its own; the lanes of a column and the wavefronts meet in LDS, in
-// order. Bound by the panels' bytes up to eight rows.
-template <int WT, int MR, int KW, int ACT>
+// sums of its own. Sums of different values change places between the halves and
+// the rows of the wavefront, so that a step adds two of them at once; then a
+// row's lanes of a column by rotations; the wavefronts meet in LDS, in order.
+// Bound by the panels' bytes: 1 x 4096 x 16384 in bf16 44.7 us, 6.0 TB/s.
+template <int WT, int MR, int KW, int U, int ACT>
 __global__ __launch_bounds__(64 * KW) void GatedStream(GatedParams p) {
   using T = typename Type<WT>::T;
   constexpr int V = 16 / sizeof(T);        // columns of a lane
   constexpr int L = kRows / V;             // lanes of a panel row
   constexpr int KR = 64 / L;               // k rows of a wavefront's read
-  constexpr int U = 4;                     // reads in flight a projection
   __shared__ float red[KW][2][MR][kRows];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -423,17 +430,31 @@ __global__ __launch_bounds__(64 * KW) void GatedStream(GatedParams p) {
           for (int c = 0; c < V; ++c) acc[g][r][c] = __builtin_fmaf(x[u][r], v[c], acc[g][r][c]);
       }
   }
-  // Sum over the lanes of a column: those that differ above log2 L.
+  // Value v = (g MR + r) V + c. After the two exchanges register j of the lanes in
+  // half b5 and odd or even row b4 holds value 4 j + 2 b4 + b5.
+  constexpr int N = 2 * MR * V;
+  float half[N / 2];
 #pragma unroll
-  for (int g = 0; g < 2; ++g)
+  for (int i = 0; i < N / 2; ++i) {
+    const int v = 2 * i;
+    const auto s = __builtin_amdgcn_permlane32_swap(
+        __float_as_uint(acc[v / (MR * V)][v / V % MR][v % V]),
+        __float_as_uint(acc[(v + 1) / (MR * V)][(v + 1) / V % MR][(v + 1) % V]), false, false);
+    half[i] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+  }
 #pragma unroll
-    for (int r = 0; r < MR; ++r)
-#pragma unroll
-      for (int c = 0; c < V; ++c) {
-        float s = acc[g][r][c];
-        for (int d = L; d < 64; d *= 2) s += ShflXor(s, d);
-        if (kr == 0) red[wave][g][r][h * V + c] = s;
-      }
+  for (int j = 0; j < N / 4; ++j) {
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(half[2 * j]),
+                                                    __float_as_uint(half[2 * j + 1]), false, false);
+    float t = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    t += Dpp<0x128>(t);
+    t += Dpp<0x124>(t);
+    if constexpr (L == 2) t += Dpp<0x122>(t);
+    if ((lane & 15) < L) {
+      const int v = 4 * j + 2 * ((lane >> 4) & 1) + (lane >> 5);
+      red[wave][v / (MR * V)][v / V % MR][h * V + v % V] = t;
+    }
+  }
   __syncthreads();
   // Thread (row, column) of the panel's results.
   for (int i = threadIdx.x; i < MR * kRows; i += 64 * KW) {
@@ -456,7 +477,8 @@ __global__ __launch_bounds__(64 * KW) void GatedStream(GatedParams p) {
 // need no cutting: a lane's weights are single words of a panel's rows, and its x
 // four consecutive k of one row, in which product i of four takes the i-th. The
 // wavefronts take 16 k in turn and meet in LDS, in order. Its products cost 2.7
-// times the planes', which the weights' bytes hide up to there.
+// times the planes', but no cutting: 80 x 4096 x 4096 57 us against the staged
+// kernel's 107 + 5 of cutting, 128 rows 94 against 106 + 5, 256 rows 174 against 153.
 template <int XP, int KW, int ACT>
 __global__ __launch_bounds__(64 * KW) void GatedDirect(GatedParams p) {
   __shared__ f32x4_t red[KW][XP * 2][64];
@@ -534,15 +556,24 @@ template <int XP, int ACT>
 hipError_t LaunchDirect(const GatedParams& p, hipStream_t stream) {
   const int64_t n = (p.x_panels + XP - 1) / XP * p.w_panels;
   if (n > INT32_MAX) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((GatedDirect<XP, 8, ACT>), dim3(static_cast<uint32_t>(n)), dim3(512), 0, stream,
-                     p);
+  // Five panels' sums leave room for four wavefronts: 80 x 4096 x 4096 57 us, 65 with
+  // eight; up to four panels eight are faster (128 rows 94 against 99).
+  constexpr int kWaves = XP > 4 ? 4 : 8;
+  hipLaunchKernelGGL((GatedDirect<XP, kWaves, ACT>), dim3(static_cast<uint32_t>(n)),
+                     dim3(64 * kWaves), 0, stream, p);
   return hipGetLastError();
 }
 
 template <int WT, int MR, int ACT>
 hipError_t LaunchStream(const GatedParams& p, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>(p.w_panels));
-  hipLaunchKernelGGL((GatedStream<WT, MR, 8, ACT>), grid, dim3(512), 0, stream, p);
+  // Eight rows' sums: four wavefronts where the panels are many (4096 x 16384 60 us,
+  // 69 with eight), eight for latency (896 x 3584 7.9 us, 8.6 with four).
+  if (MR == 8 && p.w_panels > 512)
+    hipLaunchKernelGGL((GatedStream<WT, MR, 4, 4, ACT>), grid, dim3(256), 0, stream, p);
+  else
+    hipLaunchKernelGGL((GatedStream<WT, MR, 8, MR == 1 ? 2 : 4, ACT>), grid, dim3(512), 0, stream,
+                       p);
   return hipGetLastError();
 }
 
@@ -562,45 +593,48 @@ hipError_t LaunchTiles(GatedParams p, hipStream_t stream) {
 template <int WT>
 hipError_t LaunchCut(const GatedParams& p, hipStream_t stream) {
   // A step a wavefront; for fp16, whose workgroups read all of their rows first,
-  // as many workgroups as two a CU.
-  int64_t chunks = (p.steps + 3) / 4;
-  if (WT == EHIP_WEIGHT_F16)
-    chunks = std::min(chunks, std::max<int64_t>(1, 512 / p.x_panels));
+  // no more workgroups than CUs.
+  constexpr int kWaves = WT == EHIP_WEIGHT_F16 ? kRows : 4;
+  int64_t chunks = (p.steps + kWaves - 1) / kWaves;
+  if (WT == EHIP_WEIGHT_F16) chunks = std::min(chunks, std::max<int64_t>(1, 256 / p.x_panels));
   chunks = std::min<int64_t>(chunks, 65535);
   const int chunk = static_cast<int>((p.steps + chunks - 1) / chunks);
   const dim3 grid(static_cast<uint32_t>(p.x_panels),
                   static_cast<uint32_t>((p.steps + chunk - 1) / chunk));
-  hipLaunchKernelGGL(CutRows<WT>, grid, dim3(256), 0, stream, p, chunk);
+  hipLaunchKernelGGL((CutRows<WT, kWaves>), grid, dim3(64 * kWaves), 0, stream, p, chunk);
   return hipGetLastError();
 }
 
-// The staged kernel's tile for a call, by an estimate of each one's time in us:
-// rounds of its workgroups over the chip (a part of one counts for 0.6 at least:
-// fewer workgroups on a CU run faster) times (steps times a step's time + the
-// time of filling and storing), for bf16 weights; fp16 ones take two thirds, in
-// all alike. Step times measured at 2382 x 4096 x 16384 and 64 x 4096 x 16384,
-// the rest at 2382 x 896 x 3584. What it picks (us, the tiles in the order below):
-// 2382 x 4096 x 16384 1313 of (1313, 1387, 1571, 1795), 600 rows 391 (391, 382,
-// 416, 471), 300 rows 222 (261, 236, 222, 267), 64 rows 70 (154, 110, 70, 82), 48
-// rows 59 (146, 97, 63, 59), 2382 x 896 x 3584 81 (94, 81, 81, 83).
-enum class Tile { k128x128, k128x64, k64x64, k48x32 };
+// The staged kernel's tile beside 16-bit weights: the one with the least estimated
+// time, a CU's share of the workgroups times a step's time, which is much the
+// same whether a CU runs them side by side or in turn (us a step, one
+// workgroup on a CU and a share of several). What it picks against the others (us;
+// tiles in the order below, bf16):
+//   2382 x 4096 x 16384 1313 of (1313, 1387, 1571, 2097, 1795)
+//   600 x 4096 x 16384 382 of (391, 382, 416, 539, 471)
+//   64 x 4096 x 16384 70 of (154, 110, 70, 84, 82); 48 rows 59 of (146, 97, 63, 74, 59)
+//   2382 x 896 x 3584 81 of (94, 81, 81, 88, 83); 64 rows 10.3 of (36, 22, 14, 10.3, 12.4)
+//   300 x 4096 x 4096 59 of (138, 82, 72, 71, 59)
+enum class Tile { k128x128, k128x64, k64x64, k64x32, k48x32 };
 
-Tile PickTile(const GatedParams& p) {
+Tile PickTile(const GatedParams& p, bool f16) {
   struct Cost {
     Tile tile;
-    int rows, cols;  // panels of x and of y
-    double step, fixed;
+    int rows, cols;          // panels of x and of y
+    double alone[2], share[2];  // bf16, fp16
   };
-  constexpr Cost kCosts[] = {{Tile::k128x128, 8, 8, 2.05, 25},
-                             {Tile::k128x64, 8, 4, 1.08, 7},
-                             {Tile::k64x64, 4, 4, 0.62, 2},
-                             {Tile::k48x32, 3, 2, 0.33, 2}};
+  constexpr Cost kCosts[] = {{Tile::k128x128, 8, 8, {1.13, 0.86}, {1.03, 0.76}},
+                             {Tile::k128x64, 8, 4, {0.65, 0.52}, {0.55, 0.43}},
+                             {Tile::k64x64, 4, 4, {0.34, 0.28}, {0.32, 0.26}},
+                             {Tile::k64x32, 4, 2, {0.21, 0.20}, {0.21, 0.163}},
+                             {Tile::k48x32, 3, 2, {0.28, 0.31}, {0.145, 0.121}}};
   Tile best = Tile::k128x128;
   double least = 0;
   for (const Cost& c : kCosts) {
-    const double tiles = static_cast<double>((p.x_panels + c.rows - 1) / c.rows) *
-                         static_cast<double>((p.w_panels + c.cols - 1) / c.cols);
-    const double us = std::max(0.6, tiles / 512) * (static_cast<double>(p.steps) * c.step + c.fixed);
+    const int64_t tiles =
+        (p.x_panels + c.rows - 1) / c.rows * ((p.w_panels + c.cols - 1) / c.cols);
+    const int64_t on_cu = (tiles + p.cus - 1) / p.cus;
+    const double us = static_cast<double>(on_cu) * (on_cu == 1 ? c.alone : c.share)[f16];
     if (least == 0 || us < least) {
       least = us;
       best = c.tile;
@@ -628,14 +662,19 @@ hipError_t Launch(const GatedParams& p, hipStream_t stream) {
       }
     }
     if (hipError_t e = LaunchCut<WT>(p, stream); e != hipSuccess) return e;
-    return LaunchTiles<WT, 1, 4, 8, 4, 2, ACT, 1>(p, stream);
+    // 128 x 128 from 160 of them: 1000 x 4096 x 16384 1413 against 2053 us, 600 x
+    // 4096 x 4096 358 against 347, 256 rows 355 against 153.
+    if ((p.x_panels + 7) / 8 * ((p.w_panels + 7) / 8) >= 160)
+      return LaunchTiles<WT, 1, 4, 8, 4, 2, ACT, 1>(p, stream);
+    return LaunchTiles<WT, 2, 2, 2, 2, 3, ACT, 1>(p, stream);
   } else {
     if (hipError_t e = LaunchCut<WT>(p, stream); e != hipSuccess) return e;
     constexpr bool kF16 = WT == EHIP_WEIGHT_F16;
-    switch (PickTile(p)) {
+    switch (PickTile(p, kF16)) {
       case Tile::k128x128: return LaunchTiles<WT, 1, 4, 8, 4, 2, ACT, 2>(p, stream);
       case Tile::k128x64: return LaunchTiles<WT, 2, 2, 4, 4, kF16 ? 3 : 2, ACT, 2>(p, stream);
       case Tile::k64x64: return LaunchTiles<WT, 2, 2, 2, 4, 4, ACT, 2>(p, stream);
+      case Tile::k64x32: return LaunchTiles<WT, 2, 2, 2, 2, 3, ACT, 2>(p, stream);
       default: return LaunchTiles<WT, 1, 4, 3, 2, 4, ACT, 2>(p, stream);
     }
   }

@@ -246,6 +246,7 @@ struct GatedParams {
   int32_t* row_scale;    // fp16: exponents of x's rows (workspace)
   int64_t m, k, n;
   int64_t x_panels, w_panels, steps;
+  int32_t cus;           // compute units of the device
   size_t scale_at;       // bytes of the planes, where the row scales begin
   int32_t x_vec, y_vec;  // rows are 16-byte aligned
   int32_t act;           // EHIP_ACT_*
