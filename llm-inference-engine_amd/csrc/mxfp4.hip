@@ -502,13 +502,17 @@ void MxStaged(MxGemmParams p) {
 #pragma unroll
     for (int b = 0; b < (WD ? 0 : WP); ++b)
       w[b] = *reinterpret_cast<const i32x4_t*>(buf + (XT + wc * WP + b) * kMxTileBytes + lane * 16);
+    // All operands on their way before the first product (the compiler would keep
+    // two): gated 4001 x 4096 x 16384 311 -> 303 us.
+    i32x4_t x[XP];
 #pragma unroll
-    for (int a = 0; a < XP; ++a) {
-      const i32x4_t x =
-          *reinterpret_cast<const i32x4_t*>(buf + (wr * XP + a) * kMxTileBytes + lane * 16);
+    for (int a = 0; a < XP; ++a)
+      x[a] = *reinterpret_cast<const i32x4_t*>(buf + (wr * XP + a) * kMxTileBytes + lane * 16);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int b = 0; b < WP; ++b) acc[a][b] = MxMfma<J>(w[b], sw[b], x, sx[a], acc[a][b]);
-    }
+    for (int a = 0; a < XP; ++a)
+#pragma unroll
+      for (int b = 0; b < WP; ++b) acc[a][b] = MxMfma<J>(w[b], sw[b], x[a], sx[a], acc[a][b]);
   };
   // Step t waits for its own tile's loads and meets the other wavefronts', then
   // loads tile t + NS - 1 into the buffer that step t - 1 has read. The loads
