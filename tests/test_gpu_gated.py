@@ -81,7 +81,9 @@ def _dev(gctx, a):
 SHAPES = [(1, 1, 1), (1, 64, 16), (1, 896, 300), (2, 33, 17), (4, 4096, 96), (7, 100, 129),
           (8, 512, 64), (9, 1000, 111), (16, 96, 250), (17, 64, 256), (31, 130, 257),
           (32, 896, 896), (48, 2048, 200), (64, 160, 130), (65, 999, 129), (130, 300, 70),
-          (257, 256, 250), (300, 64, 512), (600, 544, 272)]
+          (257, 256, 250), (300, 64, 512), (600, 544, 272),
+          # wide enough for each of the larger tiles
+          (48, 300, 8200), (600, 97, 4000), (1000, 33, 9002), (520, 70, 12001)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
@@ -121,7 +123,7 @@ def test_packed_gated_against_64_bits(gctx, ehip_mod, m, k, n, dtype):
 
 @pytest.mark.parametrize("m,k,n", [(1, 896, 300), (3, 100, 17), (16, 1030, 64), (33, 512, 100),
                                    (65, 700, 300), (130, 2048, 129), (300, 1111, 520),
-                                   (600, 384, 700)])
+                                   (600, 384, 700), (1000, 640, 2050), (1100, 2300, 6605)])
 def test_mxfp4_gated_against_64_bits(gctx, ehip_mod, m, k, n):
     E = ehip_mod
     rng = np.random.default_rng(m + k * n)
@@ -240,6 +242,38 @@ def test_non_finite_rows_stay_in_their_rows(gctx, ehip_mod, m, dtype):
         b.free()
 
 
+@pytest.mark.parametrize("m", [3, 20, 300])
+def test_fp16_subnormal_weights_and_rows_of_any_size(gctx, ehip_mod, m):
+    """Weights among fp16's subnormals (multiples of 2^-24) are exact; rows of x
+    from 2^-120 to 2^100, one with a spike 2^20 times the rest, keep their
+    precision: beside the module's bound the fp16 planes leave out 2^-39 of a
+    row's largest |x| a term. The up bias is zero and the gate's 64 over a zero
+    weight, so y = 64 u."""
+    E = ehip_mod
+    rng = np.random.default_rng(m)
+    k, n = 200, 90
+    x = rng.standard_normal((m, k))
+    x[0, 5] *= 2.0**20
+    x *= np.exp2(np.linspace(-120, 100, m))[:, None]
+    x = x.astype(np.float32)
+    j = rng.integers(-1023, 1024, (n, k))
+    w = (j * 2.0**-24).astype(np.float16)
+    assert np.array_equal(w.astype(np.float64), j * 2.0**-24)
+    wu = _pack(gctx, w.view(np.uint16), E.WEIGHT_F16)
+    wg = _pack(gctx, np.zeros((n, k), np.uint16), E.WEIGHT_F16)
+    dx, dy = gctx.to_device(x), gctx.alloc(4 * m * n)
+    db = gctx.to_device(np.full(n, 64, np.float32))
+    assert gctx.packed_gated_gemm(dx, m, k, wg, wu, E.WEIGHT_F16, n, db, None, 0, dy) == 0
+    gctx.sync()
+    xd, wd = x.astype(np.float64), w.astype(np.float64)
+    err = np.abs(dy.download(np.float32, (m, n)) / 64.0 - xd @ wd.T)
+    bar = k * 2.0**-23 * (np.abs(xd) @ np.abs(wd).T)
+    bar += 2.0**-39 * np.abs(xd).max(1)[:, None] * np.abs(wd).sum(1)[None]
+    assert (err <= bar + 2.0**-126).all(), float((err / (bar + 2.0**-126)).max())
+    for b in (wu, wg, dx, dy, db):
+        b.free()
+
+
 # ------------------------------------------------------ the block as one run --
 
 def _block(gctx, E, rng, m, k, n, kind):
@@ -291,13 +325,13 @@ def test_feed_forward_block(gctx, ehip_mod, kind, m, k, n):
 
 @pytest.mark.parametrize("kind", ["mxfp4", "bf16", "f32"])
 def test_captured_block_replays(tctx, ehip_mod, kind):
-    """Two captured blocks share the context's workspace. Replays after new
+    """Captured blocks share the context's workspace. Replays after new
     inputs, after eager calls of other sizes, and after the workspace has grown
     past the captured one: each is bit-identical to the eager calls."""
     from ehip import hipgraph
     E, ctx = ehip_mod, tctx()
     rng = np.random.default_rng(1)
-    blocks = [_block(ctx, E, rng, m, 896, 520, kind) for m in (5, 70)]
+    blocks = [_block(ctx, E, rng, m, 896, 520, kind) for m in (5, 70, 200, 1)]
     large = _block(ctx, E, rng, 900, 896, 2000, kind)
     stream, graphs = hipgraph.Stream(), [hipgraph.Graph() for _ in blocks]
     assert E.lib().ehip_set_stream(ctx.h, stream.h) == 0

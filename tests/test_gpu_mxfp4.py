@@ -177,26 +177,32 @@ def test_unaligned_rows_quantize_alike(gctx, ehip_mod):
 SHAPES = [(1, 32, 16), (1, 896, 896), (2, 100, 33), (15, 129, 17), (16, 512, 64), (17, 513, 65),
           (32, 640, 48), (33, 2048, 100), (48, 4096, 256), (64, 1000, 129), (65, 700, 300),
           (100, 1536, 1000), (129, 384, 272), (256, 512, 512), (257, 1111, 257), (300, 4096, 520),
-          (512, 896, 1300), (513, 160, 1030), (1100, 300, 700)]
+          (512, 896, 1300), (513, 160, 1030), (1100, 300, 700), (3, 700, 40), (4, 4200, 33),
+          (5, 4200, 33), (600, 1000, 3000)]
+# 128 x 128 tiles, and 128 x 256 ones (k from 2048 on) whose k tiles are taken in
+# turns of four, two and one.
+LARGE = [(1000, 300, 4100), (1030, 2048, 12900), (1025, 2300, 12801), (1030, 2100, 12900)]
 
 
 def _grid_matrix(rng, rows, k):
     """Codes 0, .5, 1, 1.5, 2 of both signs at scales 2^-1..2^1: products are
     multiples of 2^-4 up to 16, so sums of 2^15 of them are exact in fp32."""
-    codes = rng.integers(0, 5, (rows, mx.blocks(k), 32)) | (rng.integers(0, 2, (rows, mx.blocks(k), 32)) << 3)
-    codes = codes.astype(np.uint8)
+    shape = (rows, mx.blocks(k), 32)
+    codes = (rng.integers(0, 5, shape, dtype=np.uint8) |
+             (rng.integers(0, 2, shape, dtype=np.uint8) << 3))
     codes.reshape(rows, -1)[:, k:] = 0
     return codes, rng.integers(126, 129, (rows, mx.blocks(k))).astype(np.uint8)
 
 
-@pytest.mark.parametrize("m,k,n", SHAPES)
+@pytest.mark.parametrize("m,k,n", SHAPES + LARGE)
 def test_exact_sums_are_exact(gctx, ehip_mod, m, k, n):
     rng = np.random.default_rng(m * k + n)
     xq, wq = _grid_matrix(rng, m, k), _grid_matrix(rng, n, k)
     bias = rng.integers(-8, 9, n).astype(np.float32)
     bufs = _upload(gctx, *xq) + _upload(gctx, *wq)
     db, dy = gctx.to_device(bias), gctx.alloc(4 * m * n)
-    want = mx.values(*xq, k) @ mx.values(*wq, k).T
+    # Exact in fp32 too, whatever the order.
+    want = mx.values(*xq, k).astype(np.float32) @ mx.values(*wq, k).T.astype(np.float32)
     for b in (None, db):
         assert gctx.mxfp4_gemm(bufs[0], bufs[1], m, k, bufs[2], bufs[3], n, b, dy) == 0, \
             gctx.last_error()
