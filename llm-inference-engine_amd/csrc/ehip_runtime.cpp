@@ -1013,8 +1013,7 @@ int ehip_packed_gated_gemm(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k
     return SetError(ctx, EHIP_INVALID_ARGUMENT,
                     "gated gemm: the packed weights must be 16-byte aligned (ehip_malloc gives 256)");
   ehip::GatedParams p{};
-  p.cus = ctx->cus;
-  if (int rc = EnsureGemmWorkspace(ctx, ehip::PlanGatedGemm(m, k, n, weight_dtype, &p))) return rc;
+  if (int rc = EnsureGemmWorkspace(ctx, ehip::PlanGatedGemm(m, k, n, weight_dtype, ctx->cus, &p))) return rc;
   p.x = d_x;
   p.wp[0] = d_wp_gate;
   p.wp[1] = d_wp_up;
@@ -1023,6 +1022,7 @@ int ehip_packed_gated_gemm(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k
   p.y = d_y;
   p.xp = reinterpret_cast<uint16_t*>(ctx->d_gemm);
   p.row_scale = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(ctx->d_gemm) + p.scale_at);
+  p.part = reinterpret_cast<float*>(reinterpret_cast<char*>(ctx->d_gemm) + p.part_at);
   p.x_vec = k % 4 == 0 && Aligned(d_x, 16);
   p.y_vec = n % 4 == 0 && Aligned(d_y, 16);
   p.act = activation;

@@ -207,7 +207,8 @@ __device__ __forceinline__ void LoadUnit(const Unit& u, unsigned char* buf, uint
 // planes and panel rows go from memory straight into LDS (buffer_load ... lds, 1
 // KiB units shared out over the wavefronts), NS - 1 steps
 // ahead. The weight is the A operand and x the B operand: a lane's four results
-// are four columns of one row of y.
+// are four columns of one row of y. p.splits > 1: a workgroup takes a part of the
+// steps and leaves its sums, fragment by fragment, to GatedMerge.
 template <int WT, int WR, int WC, int XP, int WP, int NS, int ACT, int OCC>
 __global__ __launch_bounds__(64 * WR * WC) __attribute__((amdgpu_waves_per_eu(OCC)))
 void GatedStaged(GatedParams p) {
@@ -230,9 +231,10 @@ void GatedStaged(GatedParams p) {
   // Tiles in bands of 4 rows of tiles, columns outer within a band; an XCD (b
   // mod 8) takes consecutive ones, which share their panels in its L2.
   const uint32_t tiles_all = static_cast<uint32_t>(p.row_tiles) * p.col_tiles;
-  const uint32_t per = (tiles_all + 7) / 8;
-  const uint32_t tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if (tile >= tiles_all) return;
+  const uint32_t work = tiles_all * p.splits, per = (work + 7) / 8;
+  const uint32_t item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (item >= work) return;
+  const uint32_t split = item / tiles_all, tile = item - split * tiles_all;
   const uint32_t band = tile / (4u * p.col_tiles);
   const uint32_t in_band = tile - band * 4u * p.col_tiles;
   const uint32_t h = min(4u, static_cast<uint32_t>(p.row_tiles) - 4u * band);
@@ -270,10 +272,20 @@ void GatedStaged(GatedParams p) {
     }
     units[i].size = bytes - min(bytes, first);
   }
+  // The steps of the workgroup's part, from a place of its own on and round: panels
+  // are a power of two apart for usual k, and workgroups at one step of different
+  // panels would meet in few of the memory's channels (a split 48 x 4096 x 16384
+  // 70 -> 64 us; whole tiles much the same).
+  const int s0 = __builtin_amdgcn_readfirstlane(split * p.split_steps);
+  const int count = min(p.split_steps, steps - s0);
+  const int turn = ct % count;
   auto stage = [&](unsigned char* buf, int t) __attribute__((always_inline)) {
+    int at = t + turn;
+    at = at >= count ? at - count : at;
+    at = s0 + min(at, count - 1);  // past the end: any step, its sums are not taken
 #pragma unroll
     for (int i = 0; i < ND; ++i)
-      LoadUnit(units[i], buf, static_cast<uint32_t>(t), lane);
+      LoadUnit(units[i], buf, static_cast<uint32_t>(at), lane);
   };
 
   f32x4_t acc[XP][WP];
@@ -335,7 +347,7 @@ void GatedStaged(GatedParams p) {
     stage(Buffer<(S + NS - 1) % NS>(b0, b1, b2, b3), t + NS - 1);
     Fence();
     compute(Buffer<S % NS>(b0, b1, b2, b3));
-    return ++t >= steps;
+    return ++t >= count;
   };
   for (;;) {
     if (step(std::integral_constant<int, 0>{})) break;
@@ -349,6 +361,15 @@ void GatedStaged(GatedParams p) {
                                                    : kFit >= 2 && XP % 2 == 0 ? 2
                                                                               : 1;
   WaitAndMeet<0>();
+  if (p.splits > 1) {
+    f32x4_t* const to = reinterpret_cast<f32x4_t*>(p.part) +
+                        (int64_t{item} * (WR * WC) + wave) * (XP * WP * 64) + lane;
+#pragma unroll
+    for (int a = 0; a < XP; ++a)
+#pragma unroll
+      for (int b = 0; b < WP; ++b) to[(a * WP + b) * 64] = acc[a][b];
+    return;
+  }
   int down[XP];
 #pragma unroll
   for (int a = 0; a < XP; ++a)
@@ -358,6 +379,47 @@ void GatedStaged(GatedParams p) {
   StoreTile<XP, WP, PP, ACT, WT == EHIP_WEIGHT_F16>(
       p, b0 + wave * (PP * C * 256), (xp0 + wr * XP) * kRows, (wp0 + wc * WP / 2) * kRows, acc,
       down);
+}
+
+// The split tiles of one row of wavefronts (WR = 1): their sums in split order,
+// then what the staged kernel does with whole ones. A workgroup a tile.
+template <int WT, int WC, int XP, int WP, int ACT>
+__global__ __launch_bounds__(64 * WC) void GatedMerge(GatedParams p) {
+  const int lane = threadIdx.x & 63, n16 = lane & 15, q = lane >> 4;
+  const int wave = static_cast<int>(threadIdx.x >> 6);
+  const uint32_t tiles = static_cast<uint32_t>(p.row_tiles) * p.col_tiles, tile = blockIdx.x;
+  // The staged kernel's order of tiles.
+  const uint32_t band = tile / (4u * p.col_tiles);
+  const uint32_t in_band = tile - band * 4u * p.col_tiles;
+  const uint32_t h = min(4u, static_cast<uint32_t>(p.row_tiles) - 4u * band);
+  const int64_t xp0 = int64_t{4 * band + in_band % h} * XP;
+  const int64_t wp0 = int64_t{in_band / h} * (WC * WP / 2) + wave * WP / 2;
+  const int64_t stride = int64_t{tiles} * WC * XP * WP * 64;
+  const f32x4_t* const from = reinterpret_cast<const f32x4_t*>(p.part) +
+                              (int64_t{tile} * WC + wave) * (XP * WP * 64) + lane;
+#pragma unroll
+  for (int a = 0; a < XP; ++a) {
+    const int64_t row = (xp0 + a) * kRows + n16;
+    if (row >= p.m) continue;
+    const int down = WT == EHIP_WEIGHT_F16 ? p.row_scale[row] : 0;
+#pragma unroll
+    for (int b = 0; b < WP; b += 2) {
+      f32x4_t g = from[(a * WP + b) * 64], u = from[(a * WP + b + 1) * 64];
+      for (int i = 1; i < p.splits; ++i) {
+        g += from[i * stride + (a * WP + b) * 64];
+        u += from[i * stride + (a * WP + b + 1) * 64];
+      }
+      if constexpr (WT == EHIP_WEIGHT_F16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          g[i] = __builtin_amdgcn_ldexpf(g[i], down);
+          u[i] = __builtin_amdgcn_ldexpf(u[i], down);
+        }
+      }
+      const int64_t col = (wp0 + b / 2) * kRows + 4 * q;
+      StoreRow4<false>(p, row, col, Finish<ACT>(p, col, g, u));
+    }
+  }
 }
 
 // Few rows (m <= MR): a workgroup per (panel, gate and up), its KW wavefronts
@@ -581,12 +643,19 @@ template <int WT, int WR, int WC, int XP, int WP, int NS, int ACT, int OCC>
 hipError_t LaunchTiles(GatedParams p, hipStream_t stream) {
   const int64_t rt = (p.x_panels + WR * XP - 1) / (WR * XP);
   const int64_t ct = (p.w_panels + WC * WP / 2 - 1) / (WC * WP / 2);
-  if (rt * ct > (int64_t{1} << 30)) return hipErrorInvalidValue;
+  if (rt * ct * p.splits > (int64_t{1} << 30)) return hipErrorInvalidValue;
   p.row_tiles = static_cast<int32_t>(rt);
   p.col_tiles = static_cast<int32_t>(ct);
-  const uint32_t grid = static_cast<uint32_t>((rt * ct + 7) / 8 * 8);
+  const uint32_t grid = static_cast<uint32_t>((rt * ct * p.splits + 7) / 8 * 8);
   hipLaunchKernelGGL((GatedStaged<WT, WR, WC, XP, WP, NS, ACT, OCC>), dim3(grid),
                      dim3(64 * WR * WC), 0, stream, p);
+  if constexpr (WR == 1 && WC == 4 && XP <= 4 && WP == 4) {  // the split tiles
+    if (p.splits > 1) {
+      if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+      hipLaunchKernelGGL((GatedMerge<WT, WC, XP, WP, ACT>), dim3(static_cast<uint32_t>(rt * ct)),
+                         dim3(64 * WC), 0, stream, p);
+    }
+  }
   return hipGetLastError();
 }
 
@@ -603,44 +672,6 @@ hipError_t LaunchCut(const GatedParams& p, hipStream_t stream) {
                   static_cast<uint32_t>((p.steps + chunk - 1) / chunk));
   hipLaunchKernelGGL((CutRows<WT, kWaves>), grid, dim3(64 * kWaves), 0, stream, p, chunk);
   return hipGetLastError();
-}
-
-// The staged kernel's tile beside 16-bit weights: the one with the least estimated
-// time, a CU's share of the workgroups times a step's time, which is much the
-// same whether a CU runs them side by side or in turn (us a step, one
-// workgroup on a CU and a share of several). What it picks against the others (us;
-// tiles in the order below, bf16):
-//   2382 x 4096 x 16384 1313 of (1313, 1387, 1571, 2097, 1795)
-//   600 x 4096 x 16384 382 of (391, 382, 416, 539, 471)
-//   64 x 4096 x 16384 70 of (154, 110, 70, 84, 82); 48 rows 59 of (146, 97, 63, 74, 59)
-//   2382 x 896 x 3584 81 of (94, 81, 81, 88, 83); 64 rows 10.3 of (36, 22, 14, 10.3, 12.4)
-//   300 x 4096 x 4096 59 of (138, 82, 72, 71, 59)
-enum class Tile { k128x128, k128x64, k64x64, k64x32, k48x32 };
-
-Tile PickTile(const GatedParams& p, bool f16) {
-  struct Cost {
-    Tile tile;
-    int rows, cols;          // panels of x and of y
-    double alone[2], share[2];  // bf16, fp16
-  };
-  constexpr Cost kCosts[] = {{Tile::k128x128, 8, 8, {1.13, 0.86}, {1.03, 0.76}},
-                             {Tile::k128x64, 8, 4, {0.65, 0.52}, {0.55, 0.43}},
-                             {Tile::k64x64, 4, 4, {0.34, 0.28}, {0.32, 0.26}},
-                             {Tile::k64x32, 4, 2, {0.21, 0.20}, {0.21, 0.163}},
-                             {Tile::k48x32, 3, 2, {0.28, 0.31}, {0.145, 0.121}}};
-  Tile best = Tile::k128x128;
-  double least = 0;
-  for (const Cost& c : kCosts) {
-    const int64_t tiles =
-        (p.x_panels + c.rows - 1) / c.rows * ((p.w_panels + c.cols - 1) / c.cols);
-    const int64_t on_cu = (tiles + p.cus - 1) / p.cus;
-    const double us = static_cast<double>(on_cu) * (on_cu == 1 ? c.alone : c.share)[f16];
-    if (least == 0 || us < least) {
-      least = us;
-      best = c.tile;
-    }
-  }
-  return best;
 }
 
 template <int WT, int ACT>
@@ -670,12 +701,19 @@ hipError_t Launch(const GatedParams& p, hipStream_t stream) {
   } else {
     if (hipError_t e = LaunchCut<WT>(p, stream); e != hipSuccess) return e;
     constexpr bool kF16 = WT == EHIP_WEIGHT_F16;
-    switch (PickTile(p, kF16)) {
-      case Tile::k128x128: return LaunchTiles<WT, 1, 4, 8, 4, 2, ACT, 2>(p, stream);
-      case Tile::k128x64: return LaunchTiles<WT, 2, 2, 4, 4, kF16 ? 3 : 2, ACT, 2>(p, stream);
-      case Tile::k64x64: return LaunchTiles<WT, 2, 2, 2, 4, 4, ACT, 2>(p, stream);
-      case Tile::k64x32: return LaunchTiles<WT, 2, 2, 2, 2, 3, ACT, 2>(p, stream);
-      default: return LaunchTiles<WT, 1, 4, 3, 2, 4, ACT, 2>(p, stream);
+    switch (p.tile) {
+      case GatedTile::k128x128: return LaunchTiles<WT, 1, 4, 8, 4, 2, ACT, 2>(p, stream);
+      case GatedTile::k128x64: return LaunchTiles<WT, 2, 2, 4, 4, kF16 ? 3 : 2, ACT, 2>(p, stream);
+      case GatedTile::k64x64: return LaunchTiles<WT, 2, 2, 2, 4, 4, ACT, 2>(p, stream);
+      case GatedTile::k64x32: return LaunchTiles<WT, 2, 2, 2, 2, 3, ACT, 2>(p, stream);
+      case GatedTile::k48x32: return LaunchTiles<WT, 1, 4, 3, 2, 4, ACT, 2>(p, stream);
+      case GatedTile::kSplit: break;
+    }
+    switch (std::min<int64_t>(p.x_panels, 4)) {
+      case 1: return LaunchTiles<WT, 1, 4, 1, 4, 4, ACT, 1>(p, stream);
+      case 2: return LaunchTiles<WT, 1, 4, 2, 4, 4, ACT, 1>(p, stream);
+      case 3: return LaunchTiles<WT, 1, 4, 3, 4, 4, ACT, 1>(p, stream);
+      default: return LaunchTiles<WT, 1, 4, 4, 4, 4, ACT, 1>(p, stream);
     }
   }
 }
@@ -689,21 +727,92 @@ hipError_t LaunchType(const GatedParams& p, hipStream_t stream) {
   }
 }
 
+// The staged kernel's tile beside 16-bit weights: the one with the least estimated
+// time, a CU's share of the workgroups times a step's time, which is much the
+// same whether a CU runs them side by side or in turn (us a step, one
+// workgroup on a CU and a share of several). What it picks against the others (us;
+// tiles in the order below, bf16):
+//   2382 x 4096 x 16384 1313 of (1313, 1387, 1571, 2097, 1795)
+//   600 x 4096 x 16384 382 of (391, 382, 416, 539, 471)
+//   2382 x 896 x 3584 81 of (94, 81, 81, 88, 83); 64 rows 10.3 of (36, 22, 14, 10.3, 12.4)
+//   300 x 4096 x 4096 59 of (138, 82, 72, 71, 59)
+// and no less than its bytes from L2 take at 9.6 TB/s. Where few rows leave CUs
+// idle: tiles of up to 64 x 128 whose steps are cut so that most CUs have a part,
+// 0.22 us a step and 0.09 for each panel of x, no less than 6.3 TB/s, and 6 us
+// for the merge:
+//   16 x 4096 x 4096 25 of (43 at best whole), 48 rows 32 of (40), 16 x 4096 x 16384 53
+//   of (57); whole ones stay at 48 x 4096 x 16384, 64 of (64, split 66).
+void PickTile(bool f16, GatedParams* p) {
+  struct Cost {
+    GatedTile tile;
+    int rows, cols;             // panels of x and of y
+    double alone[2], share[2];  // bf16, fp16
+  };
+  constexpr Cost kCosts[] = {{GatedTile::k128x128, 8, 8, {1.13, 0.86}, {1.03, 0.76}},
+                             {GatedTile::k128x64, 8, 4, {0.65, 0.52}, {0.55, 0.43}},
+                             {GatedTile::k64x64, 4, 4, {0.34, 0.28}, {0.32, 0.26}},
+                             {GatedTile::k64x32, 4, 2, {0.21, 0.20}, {0.21, 0.163}},
+                             {GatedTile::k48x32, 3, 2, {0.28, 0.31}, {0.145, 0.121}}};
+  p->splits = 1;
+  p->split_steps = static_cast<int32_t>(p->steps);
+  double least = 0;
+  auto tiles = [&](int64_t rows, int64_t cols) {
+    return (p->x_panels + rows - 1) / rows * ((p->w_panels + cols - 1) / cols);
+  };
+  // KiB of a step from L2, over all tiles: the weights once a row of tiles, x once
+  // a column; 9.6 TB/s are 9375 KiB a us.
+  const int planes = f16 ? 2 : 3;
+  auto traffic = [&](int64_t rows, int64_t cols) {
+    return static_cast<double>(tiles(rows, cols) * (2 * cols + planes * rows) * p->steps);
+  };
+  for (const Cost& c : kCosts) {
+    const int64_t on_cu = (tiles(c.rows, c.cols) + p->cus - 1) / p->cus;
+    const double us =
+        std::max(static_cast<double>(on_cu * p->steps) * (on_cu == 1 ? c.alone : c.share)[f16],
+                 traffic(c.rows, c.cols) / 9375);
+    if (least == 0 || us < least) {
+      least = us;
+      p->tile = c.tile;
+    }
+  }
+  const int64_t rows = std::min<int64_t>(p->x_panels, 4);
+  const int64_t splits = std::min<int64_t>({p->cus / tiles(rows, 8), p->steps / 8, 8});
+  if (splits < 2) return;
+  const int64_t part = (p->steps + splits - 1) / splits;
+  const double us = std::max(static_cast<double>(part) * (0.22 + 0.09 * static_cast<double>(rows)),
+                             traffic(rows, 8) / 6152) +
+                    6;
+  if (us >= least) return;
+  p->tile = GatedTile::kSplit;
+  p->split_steps = static_cast<int32_t>(part);
+  p->splits = static_cast<int32_t>((p->steps + part - 1) / part);
+}
+
 }  // namespace
 
-size_t PlanGatedGemm(int64_t m, int64_t k, int64_t n, int weight_dtype, GatedParams* p) {
+size_t PlanGatedGemm(int64_t m, int64_t k, int64_t n, int weight_dtype, int cus, GatedParams* p) {
   p->m = m;
   p->k = k;
   p->n = n;
+  p->cus = cus;
   p->x_panels = (m + kRows - 1) / kRows;
   p->w_panels = (n + kRows - 1) / kRows;
   p->steps = (k + kStep - 1) / kStep;
+  p->splits = 1;
+  p->split_steps = static_cast<int32_t>(p->steps);
   if (m <= kStreamRows || (weight_dtype == EHIP_WEIGHT_F32 && p->x_panels <= kDirectPanels))
     return 0;
-  const int planes = weight_dtype == EHIP_WEIGHT_F16 ? 2 : 3;
-  p->scale_at = static_cast<size_t>(p->x_panels) * static_cast<size_t>(p->steps) * planes * 1024;
-  return p->scale_at +
-         (weight_dtype == EHIP_WEIGHT_F16 ? static_cast<size_t>(p->x_panels) * kRows * 4 : 0);
+  const bool f16 = weight_dtype == EHIP_WEIGHT_F16;
+  if (weight_dtype != EHIP_WEIGHT_F32) PickTile(f16, p);
+  auto whole = [](size_t bytes) { return (bytes + 255) & ~size_t{255}; };
+  p->scale_at =
+      static_cast<size_t>(p->x_panels) * static_cast<size_t>(p->steps) * (f16 ? 2 : 3) * 1024;
+  p->part_at = p->scale_at + whole(f16 ? static_cast<size_t>(p->x_panels) * kRows * 4 : 0);
+  if (p->splits == 1) return p->part_at;
+  // A split's sums: a tile's 16 slots by its panels of x, 1 KiB a block.
+  const int64_t rows = std::min<int64_t>(p->x_panels, 4);
+  const int64_t tiles = (p->x_panels + rows - 1) / rows * ((p->w_panels + 7) / 8);
+  return p->part_at + static_cast<size_t>(tiles * p->splits * 16 * rows) * 1024;
 }
 
 hipError_t LaunchGatedGemm(const GatedParams& p, int weight_dtype, hipStream_t stream) {

@@ -237,6 +237,7 @@ hipError_t LaunchPackWeightPanels(const void* w, int weight_dtype, int64_t n, in
 
 // The gated feed-forward block (gated_gemm.hip): y[m, n] = act(x wp[0]^T +
 // bias[0]) * (x wp[1]^T + bias[1]) over packed weights.
+enum class GatedTile : int32_t { k128x128, k128x64, k64x64, k64x32, k48x32, kSplit };
 struct GatedParams {
   const float* x;        // [m, k]
   const void* wp[2];     // gate and up panels [w_panels, k, 16]
@@ -246,14 +247,17 @@ struct GatedParams {
   int32_t* row_scale;    // fp16: exponents of x's rows (workspace)
   int64_t m, k, n;
   int64_t x_panels, w_panels, steps;
+  float* part;           // sums of split tiles (workspace)
   int32_t cus;           // compute units of the device
-  size_t scale_at;       // bytes of the planes, where the row scales begin
+  GatedTile tile;        // the staged kernel's, its k splits and their steps
+  int32_t splits, split_steps;
+  size_t scale_at, part_at;  // where the row scales and the split sums begin (bytes)
   int32_t x_vec, y_vec;  // rows are 16-byte aligned
   int32_t act;           // EHIP_ACT_*
   int32_t row_tiles, col_tiles;  // the staged kernel's (set at its launch)
 };
-// Sizes of a call; its workspace bytes.
-size_t PlanGatedGemm(int64_t m, int64_t k, int64_t n, int weight_dtype, GatedParams* p);
+// Sizes and tiles of a call (cus: the device's CU count); its workspace bytes.
+size_t PlanGatedGemm(int64_t m, int64_t k, int64_t n, int weight_dtype, int cus, GatedParams* p);
 hipError_t LaunchGatedGemm(const GatedParams& p, int weight_dtype, hipStream_t stream);
 
 // MXFP4 (mxfp4.hip; panel layout in mxfp4.h).

@@ -624,7 +624,7 @@ hipError_t LaunchProduct(const MxGemmParams& p, hipStream_t stream) {
   }
   if (tiles(4, 4) <= 896) return LaunchStaged<2, 2, 2, 2, 4, 0, ACT, 4>(p, stream);
   if (tiles(8, 16) >= 448 && p.tiles >= 16) return LaunchStaged<1, 4, 8, 4, 4, 2, ACT, 2>(p, stream);
-  return LaunchStaged<2, 2, 4, 4, 3, 0, ACT, 3>(p, stream);
+  return LaunchStaged<1, 4, 8, 2, 4, 2, ACT, 3>(p, stream);
 }
 
 // Workgroups of the panel conversions, 0 where a launch cannot hold them.
