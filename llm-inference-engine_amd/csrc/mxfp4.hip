@@ -354,20 +354,27 @@ __global__ __launch_bounds__(64 * KW) void MxDirect(MxGemmParams p) {
 // Many rows: a workgroup of WR x WC wavefronts per tile of WR XP x panels by WC WP
 // weight panels (gated: their even slots the gate's, the odd ones the up
 // projection's). k tiles go from memory straight into LDS (buffer_load ... lds, a
-// panel's 1 KiB an instruction), into NS buffers, NS - 1 tiles ahead; an operand
+// panel's 1 KiB an instruction), into four buffers, three tiles ahead; an operand
 // is one conflict-free 16-byte read. A wavefront's scales, one dword a panel and
-// group, come through registers a group ahead. WD > 0 (WR = 1, where no two
-// wavefronts share a weight panel): the weights go into registers instead, WD - 1
-// tiles ahead, which takes half of the traffic off LDS.
-template <int WR, int WC, int XP, int WP, int NS, int WD, int ACT, int OCC>
+// group, come through registers a group ahead. REG (WR = 1, where no two
+// wavefronts share a weight panel): the weights go into registers instead, a tile
+// ahead, which takes half of the traffic off LDS.
+//
+// Bound by the power the card may take, with the loads next: gated 4001 x 4096 x
+// 16384 (1.07 TFLOP) takes 303 us at 1.98 GHz with the matrix cores busy 40% of
+// them; without any loads it would be 216 us, and a loop of nothing but these
+// products reaches 5.8 to 6.7 PFLOP/s on random codes (8.6 on zeros). Steps to it:
+// 256 x 256 tiles of eight wavefronts 363, whole-line stores past the caches and
+// 128 x 256 tiles, two workgroups a CU, 317, weights in registers 295 to 311.
+template <int WR, int WC, int XP, int WP, bool REG, int ACT, int OCC>
 __global__ __launch_bounds__(64 * WR * WC) __attribute__((amdgpu_waves_per_eu(OCC)))
 void MxStaged(MxGemmParams p) {
   constexpr bool GATED = ACT != kPlain;
   constexpr int XT = WR * XP, WT = WC * WP;  // panels of the tile
-  constexpr int LT = XT + (WD ? 0 : WT);  // of them through LDS
-  constexpr int ND = LT / (WR * WC);      // panels a wavefront loads into it
+  constexpr int LT = XT + (REG ? 0 : WT);  // of them through LDS
+  constexpr int ND = LT / (WR * WC);       // panels a wavefront loads into it
   static_assert(ND * WR * WC == LT && WP % 2 == 0, "whole shares, pairs of slots");
-  static_assert(WD == 0 || (WR == 1 && NS == 4 && (WD == 2 || WD == 4)), "register tiles");
+  static_assert(!REG || WR == 1, "a wavefront's own weights");
   constexpr int kStage = LT * kMxTileBytes;
   constexpr int C = WP * (GATED ? 2 : 4);  // 16-byte chunks of a wavefront's row of results
   constexpr int kResults = WR * WC * C * 256;
@@ -377,7 +384,7 @@ void MxStaged(MxGemmParams p) {
   __shared__ __align__(16) unsigned char b0[kFirst];
   __shared__ __align__(16) unsigned char b1[kStage];
   __shared__ __align__(16) unsigned char b2[kStage];
-  __shared__ __align__(16) unsigned char b3[NS > 3 ? kStage : 16];
+  __shared__ __align__(16) unsigned char b3[kStage];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int wr = wave / WC, wc = wave % WC;
@@ -415,18 +422,17 @@ void MxStaged(MxGemmParams p) {
     src[i] = slot < XT ? p.xc + (xp0 + min(slot, last_x)) * row_bytes
                        : p.wc[GATED ? w & 1 : 0] + (wp0 + min(GATED ? w / 2 : w, last_w)) * row_bytes;
   }
-  const uint8_t* wsrc[WD ? WP : 1];
+  const uint8_t* wsrc[REG ? WP : 1];
 #pragma unroll
-  for (int b = 0; b < (WD ? WP : 0); ++b) {
+  for (int b = 0; b < (REG ? WP : 0); ++b) {
     const int w = wc * WP + b;
     wsrc[b] = p.wc[GATED ? w & 1 : 0] + (wp0 + min(GATED ? w / 2 : w, last_w)) * row_bytes;
   }
-  constexpr int kW = WD ? WD : 1;
-  i32x4_t wf[kW][WP];
+  i32x4_t wf[2][WP];
   auto load_w = [&](i32x4_t (&w)[WP], int t) __attribute__((always_inline)) {
     const uint32_t at = static_cast<uint32_t>(min(t ^ turn, p.tiles - 1)) * kMxTileBytes;
 #pragma unroll
-    for (int b = 0; b < (WD ? WP : 0); ++b)
+    for (int b = 0; b < (REG ? WP : 0); ++b)
       w[b] = __builtin_bit_cast(
           i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
                        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(wsrc[b]), 0,
@@ -487,20 +493,19 @@ void MxStaged(MxGemmParams p) {
   load_scales(0, nx, nw);
   Fence();
   stage(b0, 0);
-  if constexpr (WD > 0) load_w(wf[0], 0);
+  Fence();
+  if constexpr (REG) load_w(wf[0], 0);
   Fence();
   stage(b1, 1);
-  if constexpr (WD > 2) load_w(wf[1], 1);
   Fence();
-  if constexpr (NS > 3) stage(b2, 2);
-  if constexpr (WD > 2) load_w(wf[2], 2);
+  stage(b2, 2);
   Fence();
   turned(nx, nw);
   auto compute = [&](auto j, const unsigned char* buf, i32x4_t (&w)[WP])
                      __attribute__((always_inline)) {
     constexpr int J = decltype(j)::value;
 #pragma unroll
-    for (int b = 0; b < (WD ? 0 : WP); ++b)
+    for (int b = 0; b < (REG ? 0 : WP); ++b)
       w[b] = *reinterpret_cast<const i32x4_t*>(buf + (XT + wc * WP + b) * kMxTileBytes + lane * 16);
     // All operands on their way before the first product (the compiler would keep
     // two): gated 4001 x 4096 x 16384 311 -> 303 us.
@@ -515,44 +520,33 @@ void MxStaged(MxGemmParams p) {
       for (int b = 0; b < WP; ++b) acc[a][b] = MxMfma<J>(w[b], sw[b], x[a], sx[a], acc[a][b]);
   };
   // Step t waits for its own tile's loads and meets the other wavefronts', then
-  // loads tile t + NS - 1 into the buffer that step t - 1 has read. The loads
-  // stay unconditional (past the end: the last tile again), so that the counts
-  // hold: behind a tile's loads are NS - 2 more tiles', WD - 1 or more sets of
-  // weights, and the next group's scales, which step 0 of a group loads before
-  // its tile, wherever they came in between. True after the last tile.
+  // loads tile t + 3 into the buffer that step t - 1 has read. The loads stay
+  // unconditional (past the end: the last tile again), so that the counts hold:
+  // behind a tile's loads are two more tiles', a set of weights or more, and, at
+  // steps 1 and 2 of a group, the next group's scales, which step 0 loads before
+  // its tile. True after the last tile.
   int g = 0;
   auto step = [&](auto s) __attribute__((always_inline)) {
-    constexpr int S = decltype(s)::value, J = S % 4;
-    constexpr int kTiles = (NS - 2) * ND + (WD ? WD - 1 : 0) * WP;
-    constexpr int kPending = J > 0 && J < NS - 1 ? kTiles + XP + WP : kTiles;
-    WaitAndMeet<kPending>();
+    constexpr int J = decltype(s)::value;
+    constexpr int kTiles = 2 * ND + (REG ? WP : 0);
+    WaitAndMeet<(J == 1 || J == 2) ? kTiles + XP + WP : kTiles>();
     if constexpr (J == 0) {
       load_scales(g + 1, nx, nw);
       Fence();
     }
-    stage(Buffer<(S + NS - 1) % NS>(b0, b1, b2, b3), 4 * g + J + NS - 1);
-    if constexpr (WD > 0) load_w(wf[(S + WD - 1) % kW], 4 * g + J + WD - 1);
+    stage(Buffer<(J + 3) % 4>(b0, b1, b2, b3), 4 * g + J + 3);
+    Fence();  // the counts go by this order
+    if constexpr (REG) load_w(wf[(J + 1) % 2], 4 * g + J + 1);
     Fence();
-    compute(std::integral_constant<int, J>{}, Buffer<S % NS>(b0, b1, b2, b3),
-            wf[S % kW]);
+    compute(s, Buffer<J>(b0, b1, b2, b3), wf[REG ? J % 2 : 0]);
     return 4 * g + J + 1 >= p.tiles;
   };
-  auto group = [&](auto s) __attribute__((always_inline)) {
-    constexpr int S = decltype(s)::value;
-    if (step(std::integral_constant<int, S>{})) return true;
-    if (step(std::integral_constant<int, S + 1>{})) return true;
-    if (step(std::integral_constant<int, S + 2>{})) return true;
-    if (step(std::integral_constant<int, S + 3>{})) return true;
+  for (;; ++g) {
+    if (step(std::integral_constant<int, 0>{})) break;
+    if (step(std::integral_constant<int, 1>{})) break;
+    if (step(std::integral_constant<int, 2>{})) break;
+    if (step(std::integral_constant<int, 3>{})) break;
     turned(nx, nw);
-    ++g;
-    return false;
-  };
-  for (;;) {
-    if (group(std::integral_constant<int, 0>{})) break;
-    if constexpr (NS == 3) {  // twelve steps until buffer and tile of the group meet again
-      if (group(std::integral_constant<int, 4>{})) break;
-      if (group(std::integral_constant<int, 8>{})) break;
-    }
   }
 
   // Loads past the end may still be in flight into the buffers: they land first.
@@ -564,7 +558,7 @@ void MxStaged(MxGemmParams p) {
                                     unscaled);
 }
 
-template <int WR, int WC, int XP, int WP, int NS, int WD, int ACT, int OCC>
+template <int WR, int WC, int XP, int WP, bool REG, int ACT, int OCC>
 hipError_t LaunchStaged(MxGemmParams p, hipStream_t stream) {
   constexpr int64_t XT = WR * XP, WT = ACT != kPlain ? WC * WP / 2 : WC * WP;
   const int64_t rt = (p.x_panels + XT - 1) / XT, ct = (p.w_panels + WT - 1) / WT;
@@ -572,7 +566,7 @@ hipError_t LaunchStaged(MxGemmParams p, hipStream_t stream) {
   p.row_tiles = static_cast<int32_t>(rt);
   p.col_tiles = static_cast<int32_t>(ct);
   const uint32_t grid = static_cast<uint32_t>((rt * ct + 7) / 8 * 8);
-  hipLaunchKernelGGL((MxStaged<WR, WC, XP, WP, NS, WD, ACT, OCC>), dim3(grid), dim3(64 * WR * WC), 0,
+  hipLaunchKernelGGL((MxStaged<WR, WC, XP, WP, REG, ACT, OCC>), dim3(grid), dim3(64 * WR * WC), 0,
                      stream, p);
   return hipGetLastError();
 }
@@ -622,9 +616,9 @@ hipError_t LaunchProduct(const MxGemmParams& p, hipStream_t stream) {
       default: return LaunchDirect<4, ACT, false>(p, stream);
     }
   }
-  if (tiles(4, 4) <= 896) return LaunchStaged<2, 2, 2, 2, 4, 0, ACT, 4>(p, stream);
-  if (tiles(8, 16) >= 448 && p.tiles >= 16) return LaunchStaged<1, 4, 8, 4, 4, 2, ACT, 2>(p, stream);
-  return LaunchStaged<1, 4, 8, 2, 4, 2, ACT, 3>(p, stream);
+  if (tiles(4, 4) <= 896) return LaunchStaged<2, 2, 2, 2, false, ACT, 4>(p, stream);
+  if (tiles(8, 16) >= 448 && p.tiles >= 16) return LaunchStaged<1, 4, 8, 4, true, ACT, 2>(p, stream);
+  return LaunchStaged<1, 4, 8, 2, true, ACT, 3>(p, stream);
 }
 
 // Workgroups of the panel conversions, 0 where a launch cannot hold them.

@@ -274,6 +274,90 @@ def test_fp16_subnormal_weights_and_rows_of_any_size(gctx, ehip_mod, m):
         b.free()
 
 
+@pytest.mark.parametrize("m", [3, 20, 70, 300])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_bf16_planes_of_rows_of_any_size(gctx, ehip_mod, m, dtype):
+    """Rows of x from 2^-120 to 2^100 keep their precision: beside the module's
+    bound, planes below bf16's normal range may be lost, 2^-125 of |w| (of fp32
+    weights too: of |x|) a term, and a sum's subnormals, 2^-126 an addition. y =
+    64 u, as above."""
+    E = ehip_mod
+    rng = np.random.default_rng(m)
+    k, n = 200, 90
+    x = rng.standard_normal((m, k)) * np.exp2(np.linspace(-120, 100, m))[:, None]
+    x = x.astype(np.float32)
+    (ub, uv, code), (gb, _, _) = (_weight(E, rng, n, k, dtype) for _ in range(2))
+    wu, wg = _pack(gctx, ub, code), _pack(gctx, np.zeros_like(gb), code)
+    dx, dy = gctx.to_device(x), gctx.alloc(4 * m * n)
+    db = gctx.to_device(np.full(n, 64, np.float32))
+    assert gctx.packed_gated_gemm(dx, m, k, wg, wu, code, n, db, None, 0, dy) == 0
+    gctx.sync()
+    xd, wd = x.astype(np.float64), uv.astype(np.float64)
+    err = np.abs(dy.download(np.float32, (m, n)) / 64.0 - xd @ wd.T)
+    bar = k * 2.0**-23 * (np.abs(xd) @ np.abs(wd).T) + 2.0**-125 * np.abs(wd).sum(1)[None]
+    bar += (2.0**-125 * np.abs(xd).sum(1)[:, None] if dtype == "f32" else 0) + k * 2.0**-126
+    assert (err <= bar).all(), float((err / bar).max())
+    for b in (wu, wg, dx, dy, db):
+        b.free()
+
+
+@pytest.mark.parametrize("m,k,n", [(1100, 2300, 6605), (1000, 640, 4100), (2500, 2560, 4096)])
+def test_mxfp4_passes_on_other_inputs_between(gctx, ehip_mod, m, k, n):
+    """Passes that nothing waits between, on two inputs in turn: a tile that is
+    read before its loads have landed shows as another pass's values."""
+    E = ehip_mod
+    rng = np.random.default_rng(m)
+    xs = [gctx.to_device(rng.standard_normal((m, k)).astype(np.float32)) for _ in range(2)]
+    ys = [gctx.alloc(4 * m * n) for _ in range(2)]
+    wg, wu = (_quantize(gctx, E, rng.standard_normal((n, k)).astype(np.float32) / 30)
+              for _ in range(2))
+
+    def calls():
+        for dx, dy in zip(xs, ys):
+            assert gctx.mxfp4_gated_linear(dx, m, k, *wg, *wu, n, None, None, 0, dy) == 0
+
+    calls()
+    gctx.sync()
+    want = [dy.download(np.uint32, (m, n)) for dy in ys]
+    for _ in range(8):
+        for _ in range(4):
+            calls()
+        gctx.sync()
+        for dy, w in zip(ys, want):
+            assert np.array_equal(dy.download(np.uint32, (m, n)), w)
+    for b in (*xs, *ys, *wg, *wu):
+        b.free()
+
+
+def test_two_contexts_at_once(tctx, ehip_mod):
+    """Two contexts' calls run side by side on their own streams, each over its own
+    workspace: the results of either alone."""
+    E, ctxs = ehip_mod, [tctx(), tctx()]
+    sizes = [[(300, 512, 520), (20, 4096, 256)], [(257, 640, 400), (70, 4096, 264)]]
+    for kind in ("bf16", "mxfp4"):
+        rng = np.random.default_rng(7)
+        blocks = [[_block(c, E, rng, *s, kind) for s in ss] for c, ss in zip(ctxs, sizes)]
+        want = []
+        for c, bs in zip(ctxs, blocks):
+            want.append([])
+            for x, _, (_, _, dy), calls, _ in bs:
+                calls()
+                c.sync()
+                want[-1].append(dy.download(np.float32, x.shape))
+                dy.upload(np.full(x.shape, np.nan, np.float32))
+        for _ in range(20):
+            for bs in zip(*blocks):
+                for b in bs:
+                    b[3]()
+        for c, bs, ws in zip(ctxs, blocks, want):
+            c.sync()
+            for (x, _, io, _, bufs), w in zip(bs, ws):
+                got = io[2].download(np.float32, x.shape)
+                assert np.array_equal(got.view(np.uint32), w.view(np.uint32)), kind
+                for b in (*io, *bufs):
+                    b.free()
+
+
 # ------------------------------------------------------ the block as one run --
 
 def _block(gctx, E, rng, m, k, n, kind):
@@ -323,16 +407,17 @@ def test_feed_forward_block(gctx, ehip_mod, kind, m, k, n):
         b.free()
 
 
-@pytest.mark.parametrize("kind", ["mxfp4", "bf16", "f32"])
-def test_captured_block_replays(tctx, ehip_mod, kind):
+@pytest.mark.parametrize("kind,k", [("mxfp4", 896), ("bf16", 896), ("f32", 896), ("bf16", 4096),
+                                    ("f16", 4096)])  # 4096: split tiles
+def test_captured_block_replays(tctx, ehip_mod, kind, k):
     """Captured blocks share the context's workspace. Replays after new
     inputs, after eager calls of other sizes, and after the workspace has grown
     past the captured one: each is bit-identical to the eager calls."""
     from ehip import hipgraph
     E, ctx = ehip_mod, tctx()
     rng = np.random.default_rng(1)
-    blocks = [_block(ctx, E, rng, m, 896, 520, kind) for m in (5, 70, 200, 1)]
-    large = _block(ctx, E, rng, 900, 896, 2000, kind)
+    blocks = [_block(ctx, E, rng, m, k, 520, kind) for m in (5, 70, 200, 1)]
+    large = _block(ctx, E, rng, 900, k, 2000, kind)
     stream, graphs = hipgraph.Stream(), [hipgraph.Graph() for _ in blocks]
     assert E.lib().ehip_set_stream(ctx.h, stream.h) == 0
     try:
