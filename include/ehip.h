@@ -140,8 +140,13 @@ int ehip_sync(ehip_ctx* ctx);
  * Switching streams first waits (on the host) for the work already queued on
  * the current stream: a context has one descriptor arena, one split
  * workspace and one set of queue counters, so its launches must never run on
- * two streams at once. FailedPrecondition if the current stream is being
- * captured (end the capture first). No counterpart in the reference (its
+ * two streams at once (a replay of a graph captured from it counts as one).
+ * FailedPrecondition if the current stream is being captured (end the capture
+ * first). The linear layers (ehip_packed_gemm, ehip_packed_gated_gemm and the
+ * ehip_mxfp4_* calls) can be captured likewise once a call outside a capture has
+ * made the context's workspace as large as they need; else they fail with
+ * FailedPrecondition and record nothing. A workspace that a capture has used
+ * lives as long as the context. No counterpart in the reference (its
  * kernels run on the calling thread). */
 int ehip_set_stream(ehip_ctx* ctx, void* stream);
 
@@ -261,9 +266,17 @@ int ehip_packed_gemm(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k, cons
  * activation and the product in one kernel,
  *   y[m, n] = act(x Wg^T + bias_gate) * (x Wu^T + bias_up).
  * x, biases, y fp32; d_wp_gate and d_wp_up are two weights [n, k] of one type as
- * ehip_pack_weight_panels lays them out (16-byte aligned). The sums are those of
- * ehip_packed_gemm, in the same precision; results are deterministic. Biases may
- * be null; m, k, n in [1, 2^21]; y may not overlap an operand. */
+ * ehip_pack_weight_panels lays them out (16-byte aligned). Sums are fp32, in a
+ * fixed order (deterministic), biases after them. Up to 8 rows, and fp32 weights
+ * up to 128, the products are fp32 ones. Else x is cut into 16-bit planes: three of
+ * bf16, as by ehip_packed_gemm, or beside fp16 weights two of fp16, after a power
+ * of two per row; fp32 weights into three of bf16. What is left out of a term is
+ * below 2^-24 of |x||w|, and beside it 2^-39 of the row's largest |x| times |w|
+ * (fp16), or 2^-125 |w| and, for an fp32 weight, 2^-125 |x| (bf16 planes below the
+ * normal range). A value whose planes begin with an infinity (an infinity, or in
+ * bf16 a magnitude from (2 - 2^-8) 2^127 on) makes its row's, or column's, results
+ * non-finite, as a NaN does; other rows and columns keep theirs. Biases may be
+ * null; m, k, n in [1, 2^21]; y may not overlap an operand. */
 int ehip_packed_gated_gemm(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k,
                            const void* d_wp_gate, const void* d_wp_up, int32_t weight_dtype,
                            int64_t n, const float* d_bias_gate, const float* d_bias_up,
@@ -280,7 +293,7 @@ int ehip_packed_gated_gemm(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k
  *   scales [ceil(rows/16)][ceil(k/512)][64][4] bytes: entry 16 g + r, byte j is
  *          the scale of row r's block g in the group's tile j;
  * zero bytes past the rows and the blocks. Codes are 16-byte aligned, scales 4.
- * Rows and k in [1, 2^21]. No counterpart in the reference, whose weights end at
+ * Rows and k in [1, 2^21]; what a call writes may not overlap what it reads. No counterpart in the reference, whose weights end at
  * 16 bits (src/model/packed_linear.h:31-36). */
 /* Bytes of a matrix's two arrays (host only; either pointer may be NULL). */
 int ehip_mxfp4_panel_bytes(int64_t rows, int64_t k, int64_t* codes_out, int64_t* scales_out);

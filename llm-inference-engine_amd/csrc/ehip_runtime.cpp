@@ -41,7 +41,7 @@ struct ehip_ctx {
   float* d_gemm = nullptr;
   size_t d_gemm_bytes = 0;
   bool gemm_captured = false;
-  void* retired[64] = {};  // each growth is half as much again: 64 pass any memory
+  void* retired[64] = {};  // each growth is half as much again
   int n_retired = 0;
   int cus = 256;  // compute units of the device
   int32_t* d_err = nullptr;
@@ -127,12 +127,15 @@ int EnsureGemmWorkspace(ehip_ctx* ctx, size_t need) {
   if (need > ctx->d_gemm_bytes) {
     if (capturing)
       return SetError(ctx, EHIP_FAILED_PRECONDITION,
-                      "the call needs a workspace of %zu bytes, and none that large was made before "
-                      "this capture: make the call once outside it",
+                      "the call needs a workspace of %zu bytes, and none that large was made "
+                      "before this capture: make the call once outside it",
                       need);
+    if (ctx->gemm_captured && ctx->n_retired == 64)
+      return SetError(ctx, EHIP_RESOURCE_EXHAUSTED,
+                      "captured graphs hold 64 workspaces of this context already");
     const size_t bytes = std::max(need, ctx->d_gemm_bytes * 3 / 2);
     EHIP_HIP(ctx, hipStreamSynchronize(ctx->stream));  // queued calls may use the old one
-    if (ctx->d_gemm && ctx->gemm_captured && ctx->n_retired < 64)
+    if (ctx->gemm_captured)
       ctx->retired[ctx->n_retired++] = ctx->d_gemm;
     else if (ctx->d_gemm)
       EHIP_HIP(ctx, hipFree(ctx->d_gemm));
@@ -1013,7 +1016,8 @@ int ehip_packed_gated_gemm(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k
     return SetError(ctx, EHIP_INVALID_ARGUMENT,
                     "gated gemm: the packed weights must be 16-byte aligned (ehip_malloc gives 256)");
   ehip::GatedParams p{};
-  if (int rc = EnsureGemmWorkspace(ctx, ehip::PlanGatedGemm(m, k, n, weight_dtype, ctx->cus, &p))) return rc;
+  const size_t need = ehip::PlanGatedGemm(m, k, n, weight_dtype, ctx->cus, &p);
+  if (int rc = EnsureGemmWorkspace(ctx, need)) return rc;
   p.x = d_x;
   p.wp[0] = d_wp_gate;
   p.wp[1] = d_wp_up;

@@ -3,8 +3,9 @@
 //   y[m, n] = act(x Wg^T + bg) * (x Wu^T + bu),
 // x fp32, the weights fp32, bf16 or fp16 in panels [ceil(n/16), k, 16].
 //
-// Two kernels. GatedStream, for a few rows, reads the panels once and multiplies
-// in fp32 on the vector ALUs. GatedStaged, for more, is on the matrix cores: x is
+// GatedStream, for a few rows, reads the panels once and multiplies in fp32 on the
+// vector ALUs; GatedDirect takes fp32 weights and up to 128 rows in fp32 on the
+// matrix cores. GatedStaged, for more, is on the 16-bit matrix cores: x is
 // cut into 16-bit planes whose sum is the value to 2^-24 (three of bf16; beside
 // fp16 weights two of fp16, after a power of two per row that brings the row's
 // largest magnitude to 2^14), the weights as they are (bf16, fp16) or in three
@@ -30,8 +31,8 @@ typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
 typedef __attribute__((ext_vector_type(4))) short s16x4_t;
 typedef __attribute__((ext_vector_type(8))) short s16x8_t;
 
-constexpr int kStreamRows = 8;     // up to these: GatedStream
-constexpr int kDirectPanels = 8;   // up to these, fp32 weights: GatedDirect
+constexpr int kStreamRows = 8;    // up to these: GatedStream
+constexpr int kDirectPanels = 8;  // of x, up to these, fp32 weights: GatedDirect
 
 constexpr int kRows = 16;   // rows of a panel, of x or a weight
 constexpr int kStep = 32;   // k of a step
@@ -534,7 +535,7 @@ __global__ __launch_bounds__(64 * KW) void GatedStream(GatedParams p) {
   }
 }
 
-// fp32 weights and up to some hundred rows: a workgroup per (XP panels of x, gate
+// fp32 weights and up to 128 rows: a workgroup per (XP panels of x, gate
 // and up panel), on the fp32 matrix-core product of 16 x 16 x 4, whose operands
 // need no cutting: a lane's weights are single words of a panel's rows, and its x
 // four consecutive k of one row, in which product i of four takes the i-th. The
