@@ -267,15 +267,17 @@ int ehip_packed_gemm(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k, cons
  *   y[m, n] = act(x Wg^T + bias_gate) * (x Wu^T + bias_up).
  * x, biases, y fp32; d_wp_gate and d_wp_up are two weights [n, k] of one type as
  * ehip_pack_weight_panels lays them out (16-byte aligned). Sums are fp32, in a
- * fixed order (deterministic), biases after them. Up to 8 rows, and fp32 weights
- * up to 128, the products are fp32 ones. Else x is cut into 16-bit planes: three of
- * bf16, as by ehip_packed_gemm, or beside fp16 weights two of fp16, after a power
- * of two per row; fp32 weights into three of bf16. What is left out of a term is
- * below 2^-24 of |x||w|, and beside it 2^-39 of the row's largest |x| times |w|
- * (fp16), or 2^-125 |w| and, for an fp32 weight, 2^-125 |x| (bf16 planes below the
- * normal range). A value whose planes begin with an infinity (an infinity, or in
- * bf16 a magnitude from (2 - 2^-8) 2^127 on) makes its row's, or column's, results
- * non-finite, as a NaN does; other rows and columns keep theirs. Biases may be
+ * fixed order (deterministic), biases after them. Up to 8 rows, and for fp32
+ * weights where that is faster, the products are fp32 ones. Else x is cut into
+ * 16-bit planes: beside bf16 weights three of bf16, as by ehip_packed_gemm, which
+ * leave out less than 2^-24 of |x||w| a term and 2^-125 |w| (planes below bf16's
+ * normal range); beside the others two of fp16, after a power of two per row,
+ * which leave out less than 2^-23 of |x||w| and 2^-39 of the row's largest |x|
+ * times |w|. fp32 weights are cut likewise, and with the product of both second
+ * planes less than 2^-21 of |x||w| is left out. A value whose planes begin with an
+ * infinity (an infinity, or in bf16 a magnitude from (2 - 2^-8) 2^127 on) makes its
+ * row's, or column's, results non-finite, as a NaN does; other rows and columns
+ * keep theirs. Biases may be
  * null; m, k, n in [1, 2^21]; y may not overlap an operand. */
 int ehip_packed_gated_gemm(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k,
                            const void* d_wp_gate, const void* d_wp_up, int32_t weight_dtype,

@@ -1026,6 +1026,7 @@ int ehip_packed_gated_gemm(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k
   p.y = d_y;
   p.xp = reinterpret_cast<uint16_t*>(ctx->d_gemm);
   p.row_scale = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(ctx->d_gemm) + p.scale_at);
+  p.col_scale = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(ctx->d_gemm) + p.col_at);
   p.part = reinterpret_cast<float*>(reinterpret_cast<char*>(ctx->d_gemm) + p.part_at);
   p.x_vec = k % 4 == 0 && Aligned(d_x, 16);
   p.y_vec = n % 4 == 0 && Aligned(d_y, 16);

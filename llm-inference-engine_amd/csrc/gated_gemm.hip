@@ -4,15 +4,18 @@
 // x fp32, the weights fp32, bf16 or fp16 in panels [ceil(n/16), k, 16].
 //
 // GatedStream, for a few rows, reads the panels once and multiplies in fp32 on the
-// vector ALUs; GatedDirect takes fp32 weights and up to 128 rows in fp32 on the
-// matrix cores. GatedStaged, for more, is on the 16-bit matrix cores: x is
-// cut into 16-bit planes whose sum is the value to 2^-24 (three of bf16; beside
-// fp16 weights two of fp16, after a power of two per row that brings the row's
-// largest magnitude to 2^14), the weights as they are (bf16, fp16) or in three
-// bf16 planes (fp32). Products x_i w_j with i + j <= 2, smallest first, fp32 sums:
-// three matrix-core products a term for bf16 weights, two for fp16, six for
-// fp32. What is left out is below 2^-24 of |x||w| a term (fp16: and of 2^-39 of the
-// row's largest |x| times |w|).
+// vector ALUs; GatedDirect, for small calls with fp32 weights, in fp32 on the
+// matrix cores. GatedStaged, for the others, is on the 16-bit matrix cores: beside
+// bf16 weights x is cut into three bf16 planes whose sum is the value to 2^-24.
+// Beside fp16 and fp32 weights it is two fp16 planes, the value to 2^-23, after a
+// power of two per row that brings the row's largest magnitude to 2^14; fp32
+// weights are cut alike, by rows. Products x_i w_j but that of both second planes,
+// smallest first, fp32 sums: three matrix-core products a term for bf16 and fp32
+// weights, two for fp16. What fp16 planes leave out is below 2^-23 of |x||w| a term
+// and 2^-39 of the row's largest |x| times |w|; with fp32 weights below 2^-21 at
+// worst, for all of it, in the mean square some 2^-24, where a term of fp32
+// arithmetic loses 2^-25 and the k sums of fp32 that follow sqrt(k) 2^-25 or more
+// (1200 x 4096 x 4096: 6e-7 of the result, against 1.7e-6 of a plain fp32 product).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -28,11 +31,13 @@ namespace {
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
 typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4_t;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
+typedef __attribute__((ext_vector_type(2))) float f32x2_t;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
+typedef __attribute__((ext_vector_type(2))) short s16x2_t;
 typedef __attribute__((ext_vector_type(4))) short s16x4_t;
 typedef __attribute__((ext_vector_type(8))) short s16x8_t;
 
-constexpr int kStreamRows = 8;    // up to these: GatedStream
-constexpr int kDirectPanels = 8;  // of x, up to these, fp32 weights: GatedDirect
+constexpr int kStreamRows = 8;  // up to these: GatedStream
 
 constexpr int kRows = 16;   // rows of a panel, of x or a weight
 constexpr int kStep = 32;   // k of a step
@@ -42,17 +47,20 @@ struct Type;
 template <>
 struct Type<EHIP_WEIGHT_F32> {
   using T = float;
-  static constexpr int XPL = 3, WPL = 3;  // planes of x and of a weight
+  static constexpr int XPL = 2, WPL = 2;  // planes of x and of a weight
+  static constexpr bool kHalf = true;     // planes of fp16
 };
 template <>
 struct Type<EHIP_WEIGHT_BF16> {
   using T = uint16_t;
   static constexpr int XPL = 3, WPL = 1;
+  static constexpr bool kHalf = false;
 };
 template <>
 struct Type<EHIP_WEIGHT_F16> {
   using T = uint16_t;
   static constexpr int XPL = 2, WPL = 1;
+  static constexpr bool kHalf = true;
 };
 
 // A lane (n16, q) of a matrix-core operand holds eight k of a 32-k step: 4q..4q+3
@@ -68,7 +76,7 @@ template <int WT>
 __device__ __forceinline__ void Cut(float v, short (&out)[Type<WT>::XPL]) {
 #pragma unroll
   for (int i = 0; i < Type<WT>::XPL; ++i) {
-    if constexpr (WT == EHIP_WEIGHT_F16) {
+    if constexpr (Type<WT>::kHalf) {
       const _Float16 h = static_cast<_Float16>(v);
       out[i] = __builtin_bit_cast(short, h);
       v -= static_cast<float>(h);
@@ -87,21 +95,69 @@ __device__ __forceinline__ uint32_t Moved(uint32_t v) {
       __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, false));
 }
 
+// The largest of the wavefront's, as integers: the order of non-negative floats,
+// NaN and infinities on top.
+__device__ __forceinline__ uint32_t Over16And32(uint32_t v) {
+  v = max(v, __float_as_uint(ShflXor(__uint_as_float(v), 16)));
+  return max(v, __float_as_uint(ShflXor(__uint_as_float(v), 32)));
+}
+__device__ __forceinline__ uint32_t Magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+// The power of two that brings this magnitude to [2^14, 2^15); infinities and NaN
+// stay.
+__device__ __forceinline__ int Exponent(uint32_t top) {
+  const int f = static_cast<int>(top >> 23);
+  return f == 255 ? 0 : 14 + 127 - f;
+}
+
+// Column scales of an fp32 weight's panel: a thread takes four columns of every
+// 256th row.
+__device__ __forceinline__ void ScalePanel(const GatedParams& p, int64_t which, uint32_t* tops) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t part = which >= p.w_panels, panel = which - part * p.w_panels;
+  const float* const from = static_cast<const float*>(p.wp[part]) + panel * p.k * kRows;
+  uint32_t top[4] = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < p.k * 4; i += 1024) {
+    const f32x4_t a = reinterpret_cast<const f32x4_t*>(from)[i];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top[e] = max(top[e], Magnitude(a[e]));
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    top[e] = max(top[e], Moved<0x124>(top[e]));
+    top[e] = Over16And32(max(top[e], Moved<0x128>(top[e])));
+    if (lane < 4) tops[wave * kRows + 4 * lane + e] = top[e];
+  }
+  __syncthreads();
+  if (threadIdx.x < kRows) {
+    uint32_t most = 0;
+    for (int w = 0; w < 16; ++w) most = max(most, tops[w * kRows + threadIdx.x]);
+    p.col_scale[part * p.col_stride + panel * kRows + threadIdx.x] = -Exponent(most);
+  }
+}
+
 // x [m, k] into operand panels [panels][steps][planes][64 lanes][8]: zero past m
-// and k. A workgroup takes a panel's steps [chunk * blockIdx.y, ..), a wavefront a
-// step at a time; for fp16 every workgroup of a panel first finds its rows'
-// largest magnitudes.
+// and k. A workgroup takes `chunk` steps of a panel, a wavefront a step at a time;
+// for planes of fp16 every workgroup of a panel first finds its rows' largest
+// magnitudes. Beside fp32 weights further workgroups find those of the weights'
+// columns.
 template <int WT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void CutRows(GatedParams p, int chunk) {
+__global__ __launch_bounds__(64 * WAVES) void CutRows(GatedParams p, int chunk, int cuts) {
   constexpr int PL = Type<WT>::XPL;
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  const int64_t panel = blockIdx.x, row = panel * kRows + r;
+  if constexpr (WT == EHIP_WEIGHT_F32) {
+    static_assert(WT != EHIP_WEIGHT_F32 || WAVES == 16, "ScalePanel's");
+    __shared__ uint32_t tops[WAVES * kRows];
+    if (static_cast<int>(blockIdx.x) >= cuts) return ScalePanel(p, blockIdx.x - cuts, tops);
+  }
+  const uint32_t part = blockIdx.x / static_cast<uint32_t>(p.x_panels);
+  const int64_t panel = blockIdx.x - part * static_cast<uint32_t>(p.x_panels);
+  const int64_t row = panel * kRows + r;
   const float* const src = p.x + (row < p.m ? row : 0) * p.k;
   int up = 0;
-  if constexpr (WT == EHIP_WEIGHT_F16) {
-    // A wavefront a row. As integers: the order of non-negative floats, NaN and
-    // infinities on top (such a row is left as it is).
-    static_assert(WT != EHIP_WEIGHT_F16 || WAVES == kRows, "a wavefront a row");
+  if constexpr (Type<WT>::kHalf) {
+    // A wavefront a row.
+    static_assert(!Type<WT>::kHalf || WAVES == kRows, "a wavefront a row");
     __shared__ int scale[kRows];
     const int mine = threadIdx.x >> 6;
     const int64_t at = panel * kRows + mine;
@@ -113,27 +169,23 @@ __global__ __launch_bounds__(64 * WAVES) void CutRows(GatedParams p, int chunk) 
         for (int64_t kk = 4 * lane; kk < p.k; kk += 256) {
           const f32x4_t a = *reinterpret_cast<const f32x4_t*>(from + kk);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(a[e]) & 0x7FFFFFFFu);
+          for (int e = 0; e < 4; ++e) top = max(top, Magnitude(a[e]));
         }
       } else {
 #pragma unroll 4
-        for (int64_t kk = lane; kk < p.k; kk += 64)
-          top = max(top, __float_as_uint(from[kk]) & 0x7FFFFFFFu);
+        for (int64_t kk = lane; kk < p.k; kk += 64) top = max(top, Magnitude(from[kk]));
       }
     }
     top = max(top, Moved<0xB1>(top));
     top = max(top, Moved<0x4E>(top));
     top = max(top, Moved<0x141>(top));
-    top = max(top, Moved<0x128>(top));
-    top = max(top, __float_as_uint(ShflXor(__uint_as_float(top), 16)));
-    top = max(top, __float_as_uint(ShflXor(__uint_as_float(top), 32)));
-    const int f = static_cast<int>(top >> 23);
-    if (lane == 0) scale[mine] = f == 255 ? 0 : 14 + 127 - f;
+    top = Over16And32(max(top, Moved<0x128>(top)));
+    if (lane == 0) scale[mine] = Exponent(top);
     __syncthreads();
     up = scale[r];
-    if (blockIdx.y == 0 && threadIdx.x < kRows) p.row_scale[row] = -up;
+    if (part == 0 && threadIdx.x < kRows) p.row_scale[row] = -up;
   }
-  const int64_t s0 = int64_t{blockIdx.y} * chunk, s1 = min(s0 + chunk, p.steps);
+  const int64_t s0 = int64_t{part} * chunk, s1 = min(s0 + chunk, p.steps);
   for (int64_t s = s0 + (threadIdx.x >> 6); s < s1; s += WAVES) {
     float v[8];
     if constexpr (WT == EHIP_WEIGHT_F32) {
@@ -160,7 +212,7 @@ __global__ __launch_bounds__(64 * WAVES) void CutRows(GatedParams p, int chunk) 
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       short parts[PL];
-      if constexpr (WT == EHIP_WEIGHT_F16)
+      if constexpr (Type<WT>::kHalf)
         Cut<WT>(__builtin_amdgcn_ldexpf(v[e], up), parts);
       else
         Cut<WT>(v[e], parts);
@@ -181,7 +233,7 @@ __device__ __forceinline__ s16x4_t TransposedRead(const unsigned char* p) {
 
 template <int WT>
 __device__ __forceinline__ f32x4_t Mfma(s16x8_t w, s16x8_t x, f32x4_t acc) {
-  if constexpr (WT == EHIP_WEIGHT_F16)
+  if constexpr (Type<WT>::kHalf)
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w),
                                                   __builtin_bit_cast(f16x8_t, x), acc, 0, 0, 0);
   else
@@ -272,6 +324,13 @@ void GatedStaged(GatedParams p) {
                      (wp0 + min(slot / 2, last_w)) * static_cast<int64_t>(bytes) + first;
     }
     units[i].size = bytes - min(bytes, first);
+    if constexpr (WT == EHIP_WEIGHT_F32) {  // in scalar registers, as the other types' are
+      const uint64_t src = reinterpret_cast<uint64_t>(units[i].src);
+      const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(src));
+      const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(src >> 32));
+      units[i].src = reinterpret_cast<const unsigned char*>(uint64_t{hi} << 32 | lo);
+      units[i].size = __builtin_amdgcn_readfirstlane(units[i].size);
+    }
   }
   // The steps of the workgroup's part, from a place of its own on and round: panels
   // are a power of two apart for usual k, and workgroups at one step of different
@@ -294,6 +353,13 @@ void GatedStaged(GatedParams p) {
   for (int a = 0; a < XP; ++a)
 #pragma unroll
     for (int b = 0; b < WP; ++b) acc[a][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  int up[WP];  // fp32: the powers of two of the lane's columns
+  if constexpr (WT == EHIP_WEIGHT_F32) {
+#pragma unroll
+    for (int b = 0; b < WP; ++b)
+      up[b] = -p.col_scale[(b & 1) * p.col_stride +
+                           (wp0 + min((wc * WP + b) / 2, last_w)) * kRows + n16];
+  }
 
   auto compute = [&](const unsigned char* buf) __attribute__((always_inline)) {
     s16x8_t x[XP][XPL];
@@ -309,11 +375,17 @@ void GatedStaged(GatedParams p) {
       s16x8_t w[WPL];
       if constexpr (WT == EHIP_WEIGHT_F32) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          short parts[WPL];
-          Cut<WT>(reinterpret_cast<const float*>(base)[OperandK<WT>(q, e) * kRows + n16], parts);
-#pragma unroll
-          for (int j = 0; j < WPL; ++j) w[j][e] = parts[j];
+        for (int e = 0; e < 8; e += 2) {  // in pairs, as the conversions go
+          const float* const at = reinterpret_cast<const float*>(base) + n16;
+          const f32x2_t v = {__builtin_amdgcn_ldexpf(at[OperandK<WT>(q, e) * kRows], up[b]),
+                             __builtin_amdgcn_ldexpf(at[OperandK<WT>(q, e + 1) * kRows], up[b])};
+          const f16x2_t h = __builtin_convertvector(v, f16x2_t);
+          const f32x2_t left = {__builtin_fmaf(static_cast<float>(h[0]), -1.f, v[0]),
+                                __builtin_fmaf(static_cast<float>(h[1]), -1.f, v[1])};
+          const s16x2_t hi = __builtin_bit_cast(s16x2_t, h);
+          const s16x2_t lo = __builtin_bit_cast(s16x2_t, __builtin_convertvector(left, f16x2_t));
+          w[0][e] = hi[0], w[0][e + 1] = hi[1];
+          w[1][e] = lo[0], w[1][e + 1] = lo[1];
         }
       } else {
         const unsigned char* const at = base + ((4 * q + (n16 >> 2)) * kRows + 4 * (n16 & 3)) * 2;
@@ -341,6 +413,10 @@ void GatedStaged(GatedParams p) {
   Fence();
   if constexpr (NS > 3) stage(b2, 2);
   Fence();
+  if constexpr (WT == EHIP_WEIGHT_F32) {
+#pragma unroll
+    for (int b = 0; b < WP; ++b) asm volatile("" : "+v"(up[b]));  // waited for here, not in the loop
+  }
   int t = 0;
   auto step = [&](auto s) __attribute__((always_inline)) {
     constexpr int S = decltype(s)::value;
@@ -374,10 +450,10 @@ void GatedStaged(GatedParams p) {
   int down[XP];
 #pragma unroll
   for (int a = 0; a < XP; ++a)
-    down[a] = WT == EHIP_WEIGHT_F16
+    down[a] = Type<WT>::kHalf
                   ? p.row_scale[(xp0 + min(wr * XP + a, last_x)) * kRows + n16]
                   : 0;
-  StoreTile<XP, WP, PP, ACT, WT == EHIP_WEIGHT_F16>(
+  StoreTile<XP, WP, PP, ACT, WT == EHIP_WEIGHT_F32 ? 2 : Type<WT>::kHalf>(
       p, b0 + wave * (PP * C * 256), (xp0 + wr * XP) * kRows, (wp0 + wc * WP / 2) * kRows, acc,
       down);
 }
@@ -402,7 +478,7 @@ __global__ __launch_bounds__(64 * WC) void GatedMerge(GatedParams p) {
   for (int a = 0; a < XP; ++a) {
     const int64_t row = (xp0 + a) * kRows + n16;
     if (row >= p.m) continue;
-    const int down = WT == EHIP_WEIGHT_F16 ? p.row_scale[row] : 0;
+    const int down = Type<WT>::kHalf ? p.row_scale[row] : 0;
 #pragma unroll
     for (int b = 0; b < WP; b += 2) {
       f32x4_t g = from[(a * WP + b) * 64], u = from[(a * WP + b + 1) * 64];
@@ -410,14 +486,8 @@ __global__ __launch_bounds__(64 * WC) void GatedMerge(GatedParams p) {
         g += from[i * stride + (a * WP + b) * 64];
         u += from[i * stride + (a * WP + b + 1) * 64];
       }
-      if constexpr (WT == EHIP_WEIGHT_F16) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          g[i] = __builtin_amdgcn_ldexpf(g[i], down);
-          u[i] = __builtin_amdgcn_ldexpf(u[i], down);
-        }
-      }
       const int64_t col = (wp0 + b / 2) * kRows + 4 * q;
+      if constexpr (Type<WT>::kHalf) Rescale<WT == EHIP_WEIGHT_F32>(p, col, down, &g, &u);
       StoreRow4<false>(p, row, col, Finish<ACT>(p, col, g, u));
     }
   }
@@ -535,13 +605,14 @@ __global__ __launch_bounds__(64 * KW) void GatedStream(GatedParams p) {
   }
 }
 
-// fp32 weights and up to 128 rows: a workgroup per (XP panels of x, gate
+// fp32 weights and few rows or small sizes: a workgroup per (XP panels of x, gate
 // and up panel), on the fp32 matrix-core product of 16 x 16 x 4, whose operands
 // need no cutting: a lane's weights are single words of a panel's rows, and its x
 // four consecutive k of one row, in which product i of four takes the i-th. The
-// wavefronts take 16 k in turn and meet in LDS, in order. Its products cost 2.7
-// times the planes', but no cutting: 80 x 4096 x 4096 57 us against the staged
-// kernel's 107 + 5 of cutting, 128 rows 94 against 106 + 5, 256 rows 174 against 153.
+// wavefronts take 16 k in turn and meet in LDS, in order. Its products cost five
+// times the planes', but there is no cutting and no pass over the weights before:
+// 40 x 4096 x 4096 39 us, of which the weights' bytes are 28, 100 rows 91 against
+// the staged kernel's 71 + 30 before it.
 template <int XP, int KW, int ACT>
 __global__ __launch_bounds__(64 * KW) void GatedDirect(GatedParams p) {
   __shared__ f32x4_t red[KW][XP * 2][64];
@@ -662,16 +733,17 @@ hipError_t LaunchTiles(GatedParams p, hipStream_t stream) {
 
 template <int WT>
 hipError_t LaunchCut(const GatedParams& p, hipStream_t stream) {
-  // A step a wavefront; for fp16, whose workgroups read all of their rows first,
-  // no more workgroups than CUs.
-  constexpr int kWaves = WT == EHIP_WEIGHT_F16 ? kRows : 4;
+  // A step a wavefront; for planes of fp16, whose workgroups read all of their rows
+  // first, no more workgroups than CUs.
+  constexpr int kWaves = Type<WT>::kHalf ? kRows : 4;
   int64_t chunks = (p.steps + kWaves - 1) / kWaves;
-  if (WT == EHIP_WEIGHT_F16) chunks = std::min(chunks, std::max<int64_t>(1, 256 / p.x_panels));
-  chunks = std::min<int64_t>(chunks, 65535);
-  const int chunk = static_cast<int>((p.steps + chunks - 1) / chunks);
-  const dim3 grid(static_cast<uint32_t>(p.x_panels),
-                  static_cast<uint32_t>((p.steps + chunk - 1) / chunk));
-  hipLaunchKernelGGL((CutRows<WT, kWaves>), grid, dim3(64 * kWaves), 0, stream, p, chunk);
+  if (Type<WT>::kHalf) chunks = std::min(chunks, std::max<int64_t>(1, p.cus / p.x_panels));
+  const int64_t chunk = (p.steps + chunks - 1) / chunks;
+  const int64_t cuts = p.x_panels * ((p.steps + chunk - 1) / chunk);
+  const int64_t grid = cuts + (WT == EHIP_WEIGHT_F32 ? 2 * p.w_panels : 0);
+  if (grid > INT32_MAX / (64 * kWaves)) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((CutRows<WT, kWaves>), dim3(static_cast<uint32_t>(grid)), dim3(64 * kWaves), 0,
+                     stream, p, static_cast<int>(chunk), static_cast<int>(cuts));
   return hipGetLastError();
 }
 
@@ -681,8 +753,9 @@ hipError_t Launch(const GatedParams& p, hipStream_t stream) {
   if (p.m <= 2) return LaunchStream<WT, 2, ACT>(p, stream);
   if (p.m <= 4) return LaunchStream<WT, 4, ACT>(p, stream);
   if (p.m <= kStreamRows) return LaunchStream<WT, 8, ACT>(p, stream);
-  if constexpr (WT == EHIP_WEIGHT_F32) {
-    if (p.x_panels <= kDirectPanels) {
+  constexpr bool kF32 = WT == EHIP_WEIGHT_F32, kF16 = WT == EHIP_WEIGHT_F16;
+  if constexpr (kF32) {
+    if (p.tile == GatedTile::kDirect) {
       // As few groups of rows as there can be, alike.
       const int64_t groups = (p.x_panels + 4) / 5;
       switch ((p.x_panels + groups - 1) / groups) {
@@ -693,22 +766,24 @@ hipError_t Launch(const GatedParams& p, hipStream_t stream) {
         default: return LaunchDirect<5, ACT>(p, stream);
       }
     }
-    if (hipError_t e = LaunchCut<WT>(p, stream); e != hipSuccess) return e;
-    // 128 x 128 from 160 of them: 1000 x 4096 x 16384 1413 against 2053 us, 600 x
-    // 4096 x 4096 358 against 347, 256 rows 355 against 153.
-    if ((p.x_panels + 7) / 8 * ((p.w_panels + 7) / 8) >= 160)
-      return LaunchTiles<WT, 1, 4, 8, 4, 2, ACT, 1>(p, stream);
-    return LaunchTiles<WT, 2, 2, 2, 2, 3, ACT, 1>(p, stream);
+  }
+  if (hipError_t e = LaunchCut<WT>(p, stream); e != hipSuccess) return e;
+  if constexpr (kF32) {
+    switch (p.tile) {
+      case GatedTile::k256x128: return LaunchTiles<WT, 2, 4, 8, 4, 2, ACT, 2>(p, stream);
+      case GatedTile::k256x64: return LaunchTiles<WT, 2, 4, 8, 2, 2, ACT, 2>(p, stream);
+      case GatedTile::k128x64: return LaunchTiles<WT, 2, 2, 4, 4, 2, ACT, 2>(p, stream);
+      case GatedTile::k64x32: return LaunchTiles<WT, 2, 2, 2, 2, 3, ACT, 2>(p, stream);
+      default: return LaunchTiles<WT, 1, 4, 3, 2, 3, ACT, 2>(p, stream);
+    }
   } else {
-    if (hipError_t e = LaunchCut<WT>(p, stream); e != hipSuccess) return e;
-    constexpr bool kF16 = WT == EHIP_WEIGHT_F16;
     switch (p.tile) {
       case GatedTile::k128x128: return LaunchTiles<WT, 1, 4, 8, 4, 2, ACT, 2>(p, stream);
       case GatedTile::k128x64: return LaunchTiles<WT, 2, 2, 4, 4, kF16 ? 3 : 2, ACT, 2>(p, stream);
       case GatedTile::k64x64: return LaunchTiles<WT, 2, 2, 2, 4, 4, ACT, 2>(p, stream);
       case GatedTile::k64x32: return LaunchTiles<WT, 2, 2, 2, 2, 3, ACT, 2>(p, stream);
       case GatedTile::k48x32: return LaunchTiles<WT, 1, 4, 3, 2, 4, ACT, 2>(p, stream);
-      case GatedTile::kSplit: break;
+      default: break;
     }
     switch (std::min<int64_t>(p.x_panels, 4)) {
       case 1: return LaunchTiles<WT, 1, 4, 1, 4, 4, ACT, 1>(p, stream);
@@ -728,53 +803,70 @@ hipError_t LaunchType(const GatedParams& p, hipStream_t stream) {
   }
 }
 
-// The staged kernel's tile beside 16-bit weights: the one with the least estimated
+// The staged kernel's tile: the one with the least estimated
 // time, a CU's share of the workgroups times a step's time, which is much the
 // same whether a CU runs them side by side or in turn (us a step, one
 // workgroup on a CU and a share of several). What it picks against the others (us;
-// tiles in the order below, bf16):
-//   2382 x 4096 x 16384 1313 of (1313, 1387, 1571, 2097, 1795)
+// tiles in the order below):
+//   bf16, 2382 x 4096 x 16384 1313 of (1313, 1387, 1571, 2097, 1795)
 //   600 x 4096 x 16384 382 of (391, 382, 416, 539, 471)
 //   2382 x 896 x 3584 81 of (94, 81, 81, 88, 83); 64 rows 10.3 of (36, 22, 14, 10.3, 12.4)
 //   300 x 4096 x 4096 59 of (138, 82, 72, 71, 59)
+//   fp32, 2400 x 4096 x 16384 1695 of (1695, 1863, 1966, 2772, 2746)
+//   600 x 4096 x 4096 154 of (270, 154, 174, 177, 182), 1000 x 1111 300 rows 17 of
+//   (75, 45, 33, 17, 20), 4096 x 4096 106 of (269, 150, 118, 108, 106)
 // and no less than its bytes from L2 take at 9.6 TB/s. Where few rows leave CUs
-// idle: tiles of up to 64 x 128 whose steps are cut so that most CUs have a part,
-// 0.22 us a step and 0.09 for each panel of x, no less than 6.3 TB/s, and 6 us
-// for the merge:
+// idle, 16-bit weights: tiles of up to 64 x 128 whose steps are cut so that most
+// CUs have a part, 0.22 us a step and 0.09 for each panel of x, no less than 6.3
+// TB/s, and 6 us for the merge:
 //   16 x 4096 x 4096 25 of (43 at best whole), 48 rows 32 of (40), 16 x 4096 x 16384 53
 //   of (57); whole ones stay at 48 x 4096 x 16384, 64 of (64, split 66).
-void PickTile(bool f16, GatedParams* p) {
+// fp32 weights leave GatedStaged where the cutting and the reading of the columns'
+// magnitudes that come before it (9 us and 5.2 TB/s) and its tiles take longer than
+// GatedDirect, 3.2 ns for a k of each panel of x that a CU has in turn: 100 x 4096 x
+// 4096 91 us direct and 101 staged, 200 x 896 x 3584 46 and 30.
+void PickTile(int weight_dtype, GatedParams* p) {
   struct Cost {
     GatedTile tile;
     int rows, cols;             // panels of x and of y
-    double alone[2], share[2];  // bf16, fp16
+    double alone[3], share[3];  // by EHIP_WEIGHT_*; 0: not built
   };
-  constexpr Cost kCosts[] = {{GatedTile::k128x128, 8, 8, {1.13, 0.86}, {1.03, 0.76}},
-                             {GatedTile::k128x64, 8, 4, {0.65, 0.52}, {0.55, 0.43}},
-                             {GatedTile::k64x64, 4, 4, {0.34, 0.28}, {0.32, 0.26}},
-                             {GatedTile::k64x32, 4, 2, {0.21, 0.20}, {0.21, 0.163}},
-                             {GatedTile::k48x32, 3, 2, {0.28, 0.31}, {0.145, 0.121}}};
-  p->splits = 1;
-  p->split_steps = static_cast<int32_t>(p->steps);
+  constexpr Cost kCosts[] = {{GatedTile::k256x128, 16, 8, {2.15}, {2.5}},
+                             {GatedTile::k256x64, 16, 4, {1.19}, {1.42}},
+                             {GatedTile::k128x128, 8, 8, {0, 1.13, 1.03}, {0, 0.86, 0.76}},
+                             {GatedTile::k128x64, 8, 4, {0.91, 0.65, 0.55}, {0.80, 0.52, 0.43}},
+                             {GatedTile::k64x64, 4, 4, {0, 0.34, 0.32}, {0, 0.28, 0.26}},
+                             {GatedTile::k64x32, 4, 2, {0.50, 0.21, 0.21}, {0.28, 0.20, 0.163}},
+                             {GatedTile::k48x32, 3, 2, {0.58, 0.28, 0.145}, {0.215, 0.31, 0.121}}};
+  const bool f32 = weight_dtype == EHIP_WEIGHT_F32;
   double least = 0;
   auto tiles = [&](int64_t rows, int64_t cols) {
     return (p->x_panels + rows - 1) / rows * ((p->w_panels + cols - 1) / cols);
   };
   // KiB of a step from L2, over all tiles: the weights once a row of tiles, x once
   // a column; 9.6 TB/s are 9375 KiB a us.
-  const int planes = f16 ? 2 : 3;
+  const int planes = weight_dtype == EHIP_WEIGHT_BF16 ? 3 : 2, unit = f32 ? 2 : 1;
   auto traffic = [&](int64_t rows, int64_t cols) {
-    return static_cast<double>(tiles(rows, cols) * (2 * cols + planes * rows) * p->steps);
+    return static_cast<double>(tiles(rows, cols) * (2 * unit * cols + planes * rows) * p->steps);
   };
   for (const Cost& c : kCosts) {
+    if (c.share[weight_dtype] == 0) continue;
     const int64_t on_cu = (tiles(c.rows, c.cols) + p->cus - 1) / p->cus;
-    const double us =
-        std::max(static_cast<double>(on_cu * p->steps) * (on_cu == 1 ? c.alone : c.share)[f16],
-                 traffic(c.rows, c.cols) / 9375);
+    const double us = std::max(
+        static_cast<double>(on_cu * p->steps) * (on_cu == 1 ? c.alone : c.share)[weight_dtype],
+        traffic(c.rows, c.cols) / 9375);
     if (least == 0 || us < least) {
       least = us;
       p->tile = c.tile;
     }
+  }
+  if (f32) {
+    const double words = static_cast<double>(p->w_panels * kRows) * static_cast<double>(p->k);
+    const int64_t groups = (p->x_panels + 4) / 5, panels = (p->x_panels + groups - 1) / groups;
+    const int64_t rounds = (groups * p->w_panels + p->cus - 1) / p->cus;
+    const double direct = 3.2e-3 * static_cast<double>(rounds * panels * p->k);
+    if (direct < least + 9 + 8 * words / 5.2e6) p->tile = GatedTile::kDirect;
+    return;
   }
   const int64_t rows = std::min<int64_t>(p->x_panels, 4);
   const int64_t splits = std::min<int64_t>({p->cus / tiles(rows, 8), p->steps / 8, 8});
@@ -801,14 +893,16 @@ size_t PlanGatedGemm(int64_t m, int64_t k, int64_t n, int weight_dtype, int cus,
   p->steps = (k + kStep - 1) / kStep;
   p->splits = 1;
   p->split_steps = static_cast<int32_t>(p->steps);
-  if (m <= kStreamRows || (weight_dtype == EHIP_WEIGHT_F32 && p->x_panels <= kDirectPanels))
-    return 0;
-  const bool f16 = weight_dtype == EHIP_WEIGHT_F16;
-  if (weight_dtype != EHIP_WEIGHT_F32) PickTile(f16, p);
-  auto whole = [](size_t bytes) { return (bytes + 255) & ~size_t{255}; };
+  if (m <= kStreamRows) return 0;
+  PickTile(weight_dtype, p);
+  if (p->tile == GatedTile::kDirect) return 0;
+  const bool f32 = weight_dtype == EHIP_WEIGHT_F32, half = weight_dtype != EHIP_WEIGHT_BF16;
+  auto whole = [](int64_t bytes) { return (static_cast<size_t>(bytes) + 255) & ~size_t{255}; };
   p->scale_at =
-      static_cast<size_t>(p->x_panels) * static_cast<size_t>(p->steps) * (f16 ? 2 : 3) * 1024;
-  p->part_at = p->scale_at + whole(f16 ? static_cast<size_t>(p->x_panels) * kRows * 4 : 0);
+      static_cast<size_t>(p->x_panels) * static_cast<size_t>(p->steps) * (half ? 2 : 3) * 1024;
+  p->col_at = p->scale_at + whole(half ? p->x_panels * kRows * 4 : 0);
+  p->col_stride = (p->w_panels + 8) * kRows;  // a tile's panels beyond the last
+  p->part_at = p->col_at + whole(f32 ? 2 * p->col_stride * 4 : 0);
   if (p->splits == 1) return p->part_at;
   // A split's sums: a tile's 16 slots by its panels of x, 1 KiB a block.
   const int64_t rows = std::min<int64_t>(p->x_panels, 4);

@@ -237,21 +237,26 @@ hipError_t LaunchPackWeightPanels(const void* w, int weight_dtype, int64_t n, in
 
 // The gated feed-forward block (gated_gemm.hip): y[m, n] = act(x wp[0]^T +
 // bias[0]) * (x wp[1]^T + bias[1]) over packed weights.
-enum class GatedTile : int32_t { k128x128, k128x64, k64x64, k64x32, k48x32, kSplit };
+enum class GatedTile : int32_t {
+  k256x128, k256x64, k128x128, k128x64, k64x64, k64x32, k48x32, kSplit, kDirect
+};
 struct GatedParams {
   const float* x;        // [m, k]
   const void* wp[2];     // gate and up panels [w_panels, k, 16]
   const float* bias[2];  // [n] or null
   float* y;              // [m, n]
   uint16_t* xp;          // x's planes in operand panels (workspace)
-  int32_t* row_scale;    // fp16: exponents of x's rows (workspace)
+  int32_t* row_scale;    // fp16 planes: exponents of x's rows and, fp32
+  int32_t* col_scale;    // weights, of the projections' columns (workspace)
+  int64_t col_stride;    // from the gate's to the up projection's
   int64_t m, k, n;
   int64_t x_panels, w_panels, steps;
   float* part;           // sums of split tiles (workspace)
   int32_t cus;           // compute units of the device
   GatedTile tile;        // the staged kernel's, its k splits and their steps
   int32_t splits, split_steps;
-  size_t scale_at, part_at;  // where the row scales and the split sums begin (bytes)
+  // Where the row and column scales and the split sums begin (bytes).
+  size_t scale_at, col_at, part_at;
   int32_t x_vec, y_vec;  // rows are 16-byte aligned
   int32_t act;           // EHIP_ACT_*
   int32_t row_tiles, col_tiles;  // the staged kernel's (set at its launch)

@@ -553,7 +553,7 @@ void MxStaged(MxGemmParams p) {
   constexpr int kFit = kFirst / kResults, PP = kFit >= 4 ? 4 : kFit >= 2 ? 2 : 1;
   WaitAndMeet<0>();
   const int unscaled[XP] = {};
-  StoreTile<XP, WP, PP, ACT, false>(p, b0 + wave * (PP * C * 256), (xp0 + wr * XP) * kMxRows,
+  StoreTile<XP, WP, PP, ACT, 0>(p, b0 + wave * (PP * C * 256), (xp0 + wr * XP) * kMxRows,
                                     (wp0 + (GATED ? wc * WP / 2 : wc * WP)) * kMxRows, acc,
                                     unscaled);
 }

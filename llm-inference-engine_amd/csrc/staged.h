@@ -84,14 +84,32 @@ __device__ __forceinline__ void WaitAndMeet() {
 // Keeps the compiler from moving memory operations across.
 __device__ __forceinline__ void Fence() { asm volatile("" ::: "memory"); }
 
+// Four columns' sums from `col` on, 2^down times as much, and (COLS) times their
+// columns' own powers of two. P has col_scale and col_stride, whole panels and a
+// tile's width beyond them.
+template <bool COLS, class P>
+__device__ __forceinline__ void Rescale(const P& p, int64_t col, int down, f32x4_t* g, f32x4_t* u) {
+  i32x4_t dg = {down, down, down, down}, du = dg;
+  if constexpr (COLS) {
+    dg += *reinterpret_cast<const i32x4_t*>(p.col_scale + col);
+    du += *reinterpret_cast<const i32x4_t*>(p.col_scale + p.col_stride + col);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    (*g)[i] = __builtin_amdgcn_ldexpf((*g)[i], dg[i]);
+    (*u)[i] = __builtin_amdgcn_ldexpf((*u)[i], du[i]);
+  }
+}
+
 // A tile's results, acc[XP][WP] of 16 x 16 blocks (lane (n16, q): columns 4q..4q+3
 // of row n16; gated: even slots the gate's, odd ones the up projection's), from
 // row0 and col0 of y. Through `part` of LDS, the wavefront's own C * 256 * PP
 // bytes, so that a store instruction writes whole runs of its columns (256
 // bytes a row at WP = 4, gated 128) instead of 64-byte pieces of 16 rows: 16-byte
 // chunk c of row r at c ^ r, where the 16 lanes of a pass hit distinct banks.
-// SCALED: the sums of panel a's row n16 stand for 2^down[a] times as much.
-template <int XP, int WP, int PP, int ACT, bool SCALED, class P>
+// SCALED > 0: the sums of panel a's row n16 stand for 2^down[a] times as much, 2:
+// the columns' likewise.
+template <int XP, int WP, int PP, int ACT, int SCALED, class P>
 __device__ __forceinline__ void StoreTile(const P& p, unsigned char* part, int64_t row0,
                                           int64_t col0, const f32x4_t (&acc)[XP][WP],
                                           const int (&down)[XP]) {
@@ -106,13 +124,7 @@ __device__ __forceinline__ void StoreTile(const P& p, unsigned char* part, int64
       for (int b = 0; b < WP; b += PR) {
         const int c = b / PR * 4 + q;
         f32x4_t g = acc[a0 + a][b], u = acc[a0 + a][b + PR - 1];
-        if constexpr (SCALED) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            g[i] = __builtin_amdgcn_ldexpf(g[i], down[a0 + a]);
-            u[i] = __builtin_amdgcn_ldexpf(u[i], down[a0 + a]);
-          }
-        }
+        if constexpr (SCALED > 0) Rescale<SCALED == 2>(p, col0 + 4 * c, down[a0 + a], &g, &u);
         *reinterpret_cast<f32x4_t*>(part + ((a * 16 + n16) * C + ((c ^ n16) & (C - 1))) * 16) =
             Finish<ACT>(p, col0 + 4 * c, g, u);
       }

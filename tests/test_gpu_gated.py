@@ -83,7 +83,10 @@ SHAPES = [(1, 1, 1), (1, 64, 16), (1, 896, 300), (2, 33, 17), (4, 4096, 96), (7,
           (32, 896, 896), (48, 2048, 200), (64, 160, 130), (65, 999, 129), (130, 300, 70),
           (257, 256, 250), (300, 64, 512), (600, 544, 272),
           # wide enough for each of the larger tiles
-          (48, 300, 8200), (600, 97, 4000), (1000, 33, 9002), (520, 70, 12001)]
+          (48, 300, 8200), (600, 97, 4000), (1000, 33, 9002), (520, 70, 12001),
+          # and, fp32 weights, for each of theirs
+          (130, 1030, 4096), (600, 1030, 1040), (600, 200, 2600), (700, 200, 4096),
+          (1000, 96, 8000)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
@@ -148,7 +151,8 @@ def test_mxfp4_gated_against_64_bits(gctx, ehip_mod, m, k, n):
             b.free()
 
 
-@pytest.mark.parametrize("m,k,n", [(1, 128, 64), (8, 896, 100), (40, 64, 256), (300, 512, 256)])
+@pytest.mark.parametrize("m,k,n", [(1, 128, 64), (8, 896, 100), (40, 64, 256), (300, 512, 256),
+                                   (600, 1024, 1040)])
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 def test_every_plane_reaches_the_up_projection(gctx, ehip_mod, m, k, n, dtype):
     """With a zero gate weight and bias 64, act(64) = 64 exactly, so y = 64 u. x
@@ -326,6 +330,43 @@ def test_mxfp4_passes_on_other_inputs_between(gctx, ehip_mod, m, k, n):
         for dy, w in zip(ys, want):
             assert np.array_equal(dy.download(np.uint32, (m, n)), w)
     for b in (*xs, *ys, *wg, *wu):
+        b.free()
+
+
+@pytest.mark.parametrize("m,k,n", [(3, 200, 90), (20, 200, 90), (600, 1030, 1040)])
+def test_fp32_weights_of_any_size(gctx, ehip_mod, m, k, n):
+    """Rows of x from 2^-60 to 2^60 and weight rows from 2^-50 to 2^50, a spike
+    2^20 times the rest in some of each, keep their precision: beside the module's
+    bound 2^-39 of a row's largest |x|, and of a weight row's largest, a term. A
+    weight row with an infinity makes its own column non-finite. y = 64 u, as
+    above."""
+    E = ehip_mod
+    rng = np.random.default_rng(m)
+    x, w = rng.standard_normal((m, k)), rng.standard_normal((n, k))
+    x[0, 5] *= 2.0**20
+    w[7::16, 3] *= 2.0**20
+    x = (x * np.exp2(np.linspace(-60, 60, m))[:, None]).astype(np.float32)
+    w = (w * np.exp2(np.linspace(-50, 50, n))[:, None]).astype(np.float32)
+    w[12, 9] = np.inf
+    wu, wg = _pack(gctx, w, E.WEIGHT_F32), _pack(gctx, np.zeros_like(w), E.WEIGHT_F32)
+    dx, dy = gctx.to_device(x), gctx.alloc(4 * m * n)
+    db = gctx.to_device(np.full(n, 64, np.float32))
+    assert gctx.packed_gated_gemm(dx, m, k, wg, wu, E.WEIGHT_F32, n, db, None, 0, dy) == 0
+    gctx.sync()
+    got = dy.download(np.float32, (m, n)) / 64.0
+    assert not np.isfinite(got[:, 12]).any()
+    got, w = np.delete(got, 12, 1), np.delete(w, 12, 0)
+    xd, wd = np.abs(x.astype(np.float64)), np.abs(w.astype(np.float64))
+    ref = x.astype(np.float64) @ w.astype(np.float64).T
+    # The last rows' spikes reach 2^60 2^50 2^20, and 64 times that passes fp32's
+    # 2^128: such results (a factor of 2 and the bound's share aside) are infinite.
+    fits = 64 * np.abs(ref) < 2.0**127
+    assert fits.mean() > 0.9 and (64 * xd @ wd.T >= 2.0**127)[~np.isfinite(got)].all()
+    err = np.abs(np.where(fits, got - np.where(fits, ref, 0), 0))
+    bar = k * 2.0**-23 * (xd @ wd.T)
+    bar += 2.0**-39 * (xd.max(1)[:, None] * wd.sum(1)[None] + xd.sum(1)[:, None] * wd.max(1)[None])
+    assert (err <= bar + 2.0**-126).all(), float((err / bar).max())
+    for b in (wu, wg, dx, dy, db):
         b.free()
 
 
