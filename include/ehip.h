@@ -273,8 +273,10 @@ int ehip_packed_gemm(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k, cons
  * leave out less than 2^-24 of |x||w| a term and 2^-125 |w| (planes below bf16's
  * normal range); beside the others two of fp16, after a power of two per row,
  * which leave out less than 2^-23 of |x||w| and 2^-39 of the row's largest |x|
- * times |w|. fp32 weights are cut likewise, and with the product of both second
- * planes less than 2^-21 of |x||w| is left out. A value whose planes begin with an
+ * times |w|. For many rows bf16 weights go the same way, as one plane of fp16, and
+ * fp32 weights are cut like x; then 2^-39 of a weight row's largest times |x| is
+ * left out too, and with the product of both second planes (fp32) less than 2^-21
+ * of |x||w|. A value whose planes begin with an
  * infinity (an infinity, or in bf16 a magnitude from (2 - 2^-8) 2^127 on) makes its
  * row's, or column's, results non-finite, as a NaN does; other rows and columns
  * keep theirs. Biases may be

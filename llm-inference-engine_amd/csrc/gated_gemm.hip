@@ -9,9 +9,10 @@
 // bf16 weights x is cut into three bf16 planes whose sum is the value to 2^-24.
 // Beside fp16 and fp32 weights it is two fp16 planes, the value to 2^-23, after a
 // power of two per row that brings the row's largest magnitude to 2^14; fp32
-// weights are cut alike, by rows. Products x_i w_j but that of both second planes,
+// weights are cut alike, by rows, and for many rows bf16 ones become one fp16
+// plane, exact down to 2^-28 of the row's largest. Products x_i w_j but that of both second planes,
 // smallest first, fp32 sums: three matrix-core products a term for bf16 and fp32
-// weights, two for fp16. What fp16 planes leave out is below 2^-23 of |x||w| a term
+// weights, two for fp16 and for bf16 as fp16. What fp16 planes leave out is below 2^-23 of |x||w| a term
 // and 2^-39 of the row's largest |x| times |w|; with fp32 weights below 2^-21 at
 // worst, for all of it, in the mean square some 2^-24, where a term of fp32
 // arithmetic loses 2^-25 and the k sums of fp32 that follow sqrt(k) 2^-25 or more
@@ -42,25 +43,35 @@ constexpr int kStreamRows = 8;  // up to these: GatedStream
 constexpr int kRows = 16;   // rows of a panel, of x or a weight
 constexpr int kStep = 32;   // k of a step
 
+// A kernel's kind of weight: EHIP_WEIGHT_*, or bf16 taken as fp16.
+constexpr int kBf16AsF16 = 3;
+
 template <int WT>
 struct Type;
+template <>
+struct Type<kBf16AsF16> {
+  using T = uint16_t;
+  static constexpr int XPL = 2, WPL = 1;
+  static constexpr bool kHalf = true, kCols = true;
+};
 template <>
 struct Type<EHIP_WEIGHT_F32> {
   using T = float;
   static constexpr int XPL = 2, WPL = 2;  // planes of x and of a weight
-  static constexpr bool kHalf = true;     // planes of fp16
+  static constexpr bool kHalf = true;     // planes of fp16, x's rows scaled
+  static constexpr bool kCols = true;     // and the weights' rows
 };
 template <>
 struct Type<EHIP_WEIGHT_BF16> {
   using T = uint16_t;
   static constexpr int XPL = 3, WPL = 1;
-  static constexpr bool kHalf = false;
+  static constexpr bool kHalf = false, kCols = false;
 };
 template <>
 struct Type<EHIP_WEIGHT_F16> {
   using T = uint16_t;
   static constexpr int XPL = 2, WPL = 1;
-  static constexpr bool kHalf = true;
+  static constexpr bool kHalf = true, kCols = false;
 };
 
 // A lane (n16, q) of a matrix-core operand holds eight k of a 32-k step: 4q..4q+3
@@ -109,24 +120,37 @@ __device__ __forceinline__ int Exponent(uint32_t top) {
   return f == 255 ? 0 : 14 + 127 - f;
 }
 
-// Column scales of an fp32 weight's panel: a thread takes four columns of every
-// 256th row.
+// Column scales of a weight's panel: a thread takes 16 bytes of every 256th row
+// (16-bit weights: 512th).
+template <int WT>
 __device__ __forceinline__ void ScalePanel(const GatedParams& p, int64_t which, uint32_t* tops) {
+  constexpr bool kF32 = WT == EHIP_WEIGHT_F32;
+  constexpr int V = kF32 ? 4 : 8, L = kRows / V;  // columns of a thread, threads of a row
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t part = which >= p.w_panels, panel = which - part * p.w_panels;
-  const float* const from = static_cast<const float*>(p.wp[part]) + panel * p.k * kRows;
-  uint32_t top[4] = {0, 0, 0, 0};
+  const i32x4_t* const from =
+      reinterpret_cast<const i32x4_t*>(p.wp[part]) + panel * p.k * L;
+  uint32_t top[V] = {};
 #pragma unroll 4
-  for (int64_t i = threadIdx.x; i < p.k * 4; i += 1024) {
-    const f32x4_t a = reinterpret_cast<const f32x4_t*>(from)[i];
+  for (int64_t i = threadIdx.x; i < p.k * L; i += 1024) {
+    const i32x4_t a = from[i];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) top[e] = max(top[e], Magnitude(a[e]));
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t u = static_cast<uint32_t>(a[e]);
+      if constexpr (kF32) {
+        top[e] = max(top[e], u & 0x7FFFFFFFu);
+      } else {
+        top[2 * e] = max(top[2 * e], u << 16 & 0x7FFFFFFFu);
+        top[2 * e + 1] = max(top[2 * e + 1], u & 0x7FFF0000u);
+      }
+    }
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < V; ++e) {
+    if constexpr (L == 2) top[e] = max(top[e], Moved<0x122>(top[e]));
     top[e] = max(top[e], Moved<0x124>(top[e]));
     top[e] = Over16And32(max(top[e], Moved<0x128>(top[e])));
-    if (lane < 4) tops[wave * kRows + 4 * lane + e] = top[e];
+    if (lane < L) tops[wave * kRows + V * lane + e] = top[e];
   }
   __syncthreads();
   if (threadIdx.x < kRows) {
@@ -145,10 +169,10 @@ template <int WT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void CutRows(GatedParams p, int chunk, int cuts) {
   constexpr int PL = Type<WT>::XPL;
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  if constexpr (WT == EHIP_WEIGHT_F32) {
-    static_assert(WT != EHIP_WEIGHT_F32 || WAVES == 16, "ScalePanel's");
+  if constexpr (Type<WT>::kCols) {
+    static_assert(!Type<WT>::kCols || WAVES == 16, "ScalePanel's");
     __shared__ uint32_t tops[WAVES * kRows];
-    if (static_cast<int>(blockIdx.x) >= cuts) return ScalePanel(p, blockIdx.x - cuts, tops);
+    if (static_cast<int>(blockIdx.x) >= cuts) return ScalePanel<WT>(p, blockIdx.x - cuts, tops);
   }
   const uint32_t part = blockIdx.x / static_cast<uint32_t>(p.x_panels);
   const int64_t panel = blockIdx.x - part * static_cast<uint32_t>(p.x_panels);
@@ -353,8 +377,8 @@ void GatedStaged(GatedParams p) {
   for (int a = 0; a < XP; ++a)
 #pragma unroll
     for (int b = 0; b < WP; ++b) acc[a][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  int up[WP];  // fp32: the powers of two of the lane's columns
-  if constexpr (WT == EHIP_WEIGHT_F32) {
+  int up[WP];  // kCols: the powers of two of the lane's columns
+  if constexpr (Type<WT>::kCols) {
 #pragma unroll
     for (int b = 0; b < WP; ++b)
       up[b] = -p.col_scale[(b & 1) * p.col_stride +
@@ -391,6 +415,18 @@ void GatedStaged(GatedParams p) {
         const unsigned char* const at = base + ((4 * q + (n16 >> 2)) * kRows + 4 * (n16 & 3)) * 2;
         w[0] = __builtin_shufflevector(TransposedRead(at), TransposedRead(at + 16 * kRows * 2), 0,
                                        1, 2, 3, 4, 5, 6, 7);
+        if constexpr (WT == kBf16AsF16) {
+          const i32x4_t two = __builtin_bit_cast(i32x4_t, w[0]);
+          i32x4_t halves;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t u = static_cast<uint32_t>(two[e]);
+            const f32x2_t v = {__builtin_amdgcn_ldexpf(Bf16Lo(u), up[b]),
+                               __builtin_amdgcn_ldexpf(Bf16Hi(u), up[b])};
+            halves[e] = __builtin_bit_cast(int, __builtin_convertvector(v, f16x2_t));
+          }
+          w[0] = __builtin_bit_cast(s16x8_t, halves);
+        }
       }
       // Products x_i w_j with i + j < planes of x, smallest first.
 #pragma unroll
@@ -413,7 +449,7 @@ void GatedStaged(GatedParams p) {
   Fence();
   if constexpr (NS > 3) stage(b2, 2);
   Fence();
-  if constexpr (WT == EHIP_WEIGHT_F32) {
+  if constexpr (Type<WT>::kCols) {
 #pragma unroll
     for (int b = 0; b < WP; ++b) asm volatile("" : "+v"(up[b]));  // waited for here, not in the loop
   }
@@ -453,7 +489,7 @@ void GatedStaged(GatedParams p) {
     down[a] = Type<WT>::kHalf
                   ? p.row_scale[(xp0 + min(wr * XP + a, last_x)) * kRows + n16]
                   : 0;
-  StoreTile<XP, WP, PP, ACT, WT == EHIP_WEIGHT_F32 ? 2 : Type<WT>::kHalf>(
+  StoreTile<XP, WP, PP, ACT, Type<WT>::kCols ? 2 : Type<WT>::kHalf>(
       p, b0 + wave * (PP * C * 256), (xp0 + wr * XP) * kRows, (wp0 + wc * WP / 2) * kRows, acc,
       down);
 }
@@ -487,7 +523,7 @@ __global__ __launch_bounds__(64 * WC) void GatedMerge(GatedParams p) {
         u += from[i * stride + (a * WP + b + 1) * 64];
       }
       const int64_t col = (wp0 + b / 2) * kRows + 4 * q;
-      if constexpr (Type<WT>::kHalf) Rescale<WT == EHIP_WEIGHT_F32>(p, col, down, &g, &u);
+      if constexpr (Type<WT>::kHalf) Rescale<Type<WT>::kCols>(p, col, down, &g, &u);
       StoreRow4<false>(p, row, col, Finish<ACT>(p, col, g, u));
     }
   }
@@ -740,7 +776,7 @@ hipError_t LaunchCut(const GatedParams& p, hipStream_t stream) {
   if (Type<WT>::kHalf) chunks = std::min(chunks, std::max<int64_t>(1, p.cus / p.x_panels));
   const int64_t chunk = (p.steps + chunks - 1) / chunks;
   const int64_t cuts = p.x_panels * ((p.steps + chunk - 1) / chunk);
-  const int64_t grid = cuts + (WT == EHIP_WEIGHT_F32 ? 2 * p.w_panels : 0);
+  const int64_t grid = cuts + (Type<WT>::kCols ? 2 * p.w_panels : 0);
   if (grid > INT32_MAX / (64 * kWaves)) return hipErrorInvalidValue;
   hipLaunchKernelGGL((CutRows<WT, kWaves>), dim3(static_cast<uint32_t>(grid)), dim3(64 * kWaves), 0,
                      stream, p, static_cast<int>(chunk), static_cast<int>(cuts));
@@ -765,6 +801,12 @@ hipError_t Launch(const GatedParams& p, hipStream_t stream) {
         case 4: return LaunchDirect<4, ACT>(p, stream);
         default: return LaunchDirect<5, ACT>(p, stream);
       }
+    }
+  }
+  if constexpr (WT == EHIP_WEIGHT_BF16) {
+    if (p.tile == GatedTile::kAsF16) {
+      if (hipError_t e = LaunchCut<kBf16AsF16>(p, stream); e != hipSuccess) return e;
+      return LaunchTiles<kBf16AsF16, 1, 4, 8, 4, 2, ACT, 2>(p, stream);
     }
   }
   if (hipError_t e = LaunchCut<WT>(p, stream); e != hipSuccess) return e;
@@ -821,6 +863,10 @@ hipError_t LaunchType(const GatedParams& p, hipStream_t stream) {
 // TB/s, and 6 us for the merge:
 //   16 x 4096 x 4096 25 of (43 at best whole), 48 rows 32 of (40), 16 x 4096 x 16384 53
 //   of (57); whole ones stay at 48 x 4096 x 16384, 64 of (64, split 66).
+// bf16 weights go as fp16 (their 8 bits fit, after a power of two per row) where
+// the third product costs more than a pass over them, 5.6 TB/s, and the
+// conversions: 2382 x 4096 x 16384 1100 + 68 of cutting and pass for 1313 + 21, 2382
+// x 4096 x 4096 327 + 36 for 379 + 21, 600 x 4096 x 16384 341 + 54 for 416 + 7.
 // fp32 weights leave GatedStaged where the cutting and the reading of the columns'
 // magnitudes that come before it (9 us and 5.2 TB/s) and its tiles take longer than
 // GatedDirect, 3.2 ns for a k of each panel of x that a CU has in turn: 100 x 4096 x
@@ -860,6 +906,15 @@ void PickTile(int weight_dtype, GatedParams* p) {
       p->tile = c.tile;
     }
   }
+  if (weight_dtype == EHIP_WEIGHT_BF16) {
+    const int64_t on_cu = (tiles(8, 8) + p->cus - 1) / p->cus;
+    const double pass = static_cast<double>(p->w_panels * kRows * 4) * static_cast<double>(p->k);
+    const double us = static_cast<double>(on_cu * p->steps) * (on_cu == 1 ? 1.05 : 0.70);
+    if (us + pass / 5.6e6 + 2 < least) {
+      p->tile = GatedTile::kAsF16;
+      return;
+    }
+  }
   if (f32) {
     const double words = static_cast<double>(p->w_panels * kRows) * static_cast<double>(p->k);
     const int64_t groups = (p->x_panels + 4) / 5, panels = (p->x_panels + groups - 1) / groups;
@@ -896,13 +951,15 @@ size_t PlanGatedGemm(int64_t m, int64_t k, int64_t n, int weight_dtype, int cus,
   if (m <= kStreamRows) return 0;
   PickTile(weight_dtype, p);
   if (p->tile == GatedTile::kDirect) return 0;
-  const bool f32 = weight_dtype == EHIP_WEIGHT_F32, half = weight_dtype != EHIP_WEIGHT_BF16;
+  const bool as_f16 = p->tile == GatedTile::kAsF16;
+  const bool half = weight_dtype != EHIP_WEIGHT_BF16 || as_f16;  // planes of fp16
+  const bool cols = weight_dtype == EHIP_WEIGHT_F32 || as_f16;
   auto whole = [](int64_t bytes) { return (static_cast<size_t>(bytes) + 255) & ~size_t{255}; };
   p->scale_at =
       static_cast<size_t>(p->x_panels) * static_cast<size_t>(p->steps) * (half ? 2 : 3) * 1024;
   p->col_at = p->scale_at + whole(half ? p->x_panels * kRows * 4 : 0);
   p->col_stride = (p->w_panels + 8) * kRows;  // a tile's panels beyond the last
-  p->part_at = p->col_at + whole(f32 ? 2 * p->col_stride * 4 : 0);
+  p->part_at = p->col_at + whole(cols ? 2 * p->col_stride * 4 : 0);
   if (p->splits == 1) return p->part_at;
   // A split's sums: a tile's 16 slots by its panels of x, 1 KiB a block.
   const int64_t rows = std::min<int64_t>(p->x_panels, 4);

@@ -238,7 +238,7 @@ hipError_t LaunchPackWeightPanels(const void* w, int weight_dtype, int64_t n, in
 // The gated feed-forward block (gated_gemm.hip): y[m, n] = act(x wp[0]^T +
 // bias[0]) * (x wp[1]^T + bias[1]) over packed weights.
 enum class GatedTile : int32_t {
-  k256x128, k256x64, k128x128, k128x64, k64x64, k64x32, k48x32, kSplit, kDirect
+  k256x128, k256x64, k128x128, k128x64, k64x64, k64x32, k48x32, kAsF16, kSplit, kDirect
 };
 struct GatedParams {
   const float* x;        // [m, k]
@@ -246,8 +246,8 @@ struct GatedParams {
   const float* bias[2];  // [n] or null
   float* y;              // [m, n]
   uint16_t* xp;          // x's planes in operand panels (workspace)
-  int32_t* row_scale;    // fp16 planes: exponents of x's rows and, fp32
-  int32_t* col_scale;    // weights, of the projections' columns (workspace)
+  int32_t* row_scale;    // fp16 planes: exponents of x's rows and, fp32 weights
+  int32_t* col_scale;    // and bf16 as fp16, of the projections' columns (workspace)
   int64_t col_stride;    // from the gate's to the up projection's
   int64_t m, k, n;
   int64_t x_panels, w_panels, steps;

@@ -86,7 +86,9 @@ SHAPES = [(1, 1, 1), (1, 64, 16), (1, 896, 300), (2, 33, 17), (4, 4096, 96), (7,
           (48, 300, 8200), (600, 97, 4000), (1000, 33, 9002), (520, 70, 12001),
           # and, fp32 weights, for each of theirs
           (130, 1030, 4096), (600, 1030, 1040), (600, 200, 2600), (700, 200, 4096),
-          (1000, 96, 8000)]
+          (1000, 96, 8000),
+          # bf16 as fp16
+          (1300, 1001, 2600)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
@@ -152,7 +154,7 @@ def test_mxfp4_gated_against_64_bits(gctx, ehip_mod, m, k, n):
 
 
 @pytest.mark.parametrize("m,k,n", [(1, 128, 64), (8, 896, 100), (40, 64, 256), (300, 512, 256),
-                                   (600, 1024, 1040)])
+                                   (600, 1024, 1040), (1300, 1024, 2600)])
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 def test_every_plane_reaches_the_up_projection(gctx, ehip_mod, m, k, n, dtype):
     """With a zero gate weight and bias 64, act(64) = 64 exactly, so y = 64 u. x
@@ -333,8 +335,10 @@ def test_mxfp4_passes_on_other_inputs_between(gctx, ehip_mod, m, k, n):
         b.free()
 
 
-@pytest.mark.parametrize("m,k,n", [(3, 200, 90), (20, 200, 90), (600, 1030, 1040)])
-def test_fp32_weights_of_any_size(gctx, ehip_mod, m, k, n):
+@pytest.mark.parametrize("m,k,n,dtype", [(3, 200, 90, "f32"), (20, 200, 90, "f32"),
+                                         (600, 1030, 1040, "f32"), (20, 200, 90, "bf16"),
+                                         (1300, 1030, 2600, "bf16")])
+def test_weights_of_any_size(gctx, ehip_mod, m, k, n, dtype):
     """Rows of x from 2^-60 to 2^60 and weight rows from 2^-50 to 2^50, a spike
     2^20 times the rest in some of each, keep their precision: beside the module's
     bound 2^-39 of a row's largest |x|, and of a weight row's largest, a term. A
@@ -348,10 +352,14 @@ def test_fp32_weights_of_any_size(gctx, ehip_mod, m, k, n):
     x = (x * np.exp2(np.linspace(-60, 60, m))[:, None]).astype(np.float32)
     w = (w * np.exp2(np.linspace(-50, 50, n))[:, None]).astype(np.float32)
     w[12, 9] = np.inf
-    wu, wg = _pack(gctx, w, E.WEIGHT_F32), _pack(gctx, np.zeros_like(w), E.WEIGHT_F32)
+    bits, code = w, E.WEIGHT_F32
+    if dtype == "bf16":
+        bits, code = (w.view(np.uint32) >> 16).astype(np.uint16), E.WEIGHT_BF16
+        w = (bits.astype(np.uint32) << 16).view(np.float32)
+    wu, wg = _pack(gctx, bits, code), _pack(gctx, np.zeros_like(bits), code)
     dx, dy = gctx.to_device(x), gctx.alloc(4 * m * n)
     db = gctx.to_device(np.full(n, 64, np.float32))
-    assert gctx.packed_gated_gemm(dx, m, k, wg, wu, E.WEIGHT_F32, n, db, None, 0, dy) == 0
+    assert gctx.packed_gated_gemm(dx, m, k, wg, wu, code, n, db, None, 0, dy) == 0
     gctx.sync()
     got = dy.download(np.float32, (m, n)) / 64.0
     assert not np.isfinite(got[:, 12]).any()
