@@ -267,8 +267,8 @@ int ehip_packed_gemm(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k, cons
  *   y[m, n] = act(x Wg^T + bias_gate) * (x Wu^T + bias_up).
  * x, biases, y fp32; d_wp_gate and d_wp_up are two weights [n, k] of one type as
  * ehip_pack_weight_panels lays them out (16-byte aligned). Sums are fp32, in a
- * fixed order (deterministic), biases after them. Up to 8 rows, and for fp32
- * weights where that is faster, the products are fp32 ones. Else x is cut into
+ * fixed order (deterministic), biases after them. Up to 8 rows, and where
+ * that is faster, the products are fp32 ones. Else x is cut into
  * 16-bit planes: beside bf16 weights three of bf16, as by ehip_packed_gemm, which
  * leave out less than 2^-24 of |x||w| a term and 2^-125 |w| (planes below bf16's
  * normal range); beside the others two of fp16, after a power of two per row,

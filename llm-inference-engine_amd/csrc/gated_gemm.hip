@@ -4,19 +4,18 @@
 // x fp32, the weights fp32, bf16 or fp16 in panels [ceil(n/16), k, 16].
 //
 // GatedStream, for a few rows, reads the panels once and multiplies in fp32 on the
-// vector ALUs; GatedDirect, for small calls with fp32 weights, in fp32 on the
-// matrix cores. GatedStaged, for the others, is on the 16-bit matrix cores: beside
-// bf16 weights x is cut into three bf16 planes whose sum is the value to 2^-24.
-// Beside fp16 and fp32 weights it is two fp16 planes, the value to 2^-23, after a
-// power of two per row that brings the row's largest magnitude to 2^14; fp32
-// weights are cut alike, by rows, and for many rows bf16 ones become one fp16
-// plane, exact down to 2^-28 of the row's largest. Products x_i w_j but that of both second planes,
-// smallest first, fp32 sums: three matrix-core products a term for bf16 and fp32
-// weights, two for fp16 and for bf16 as fp16. What fp16 planes leave out is below 2^-23 of |x||w| a term
-// and 2^-39 of the row's largest |x| times |w|; with fp32 weights below 2^-21 at
-// worst, for all of it, in the mean square some 2^-24, where a term of fp32
-// arithmetic loses 2^-25 and the k sums of fp32 that follow sqrt(k) 2^-25 or more
-// (1200 x 4096 x 4096: 6e-7 of the result, against 1.7e-6 of a plain fp32 product).
+// vector ALUs; GatedDirect, for small calls, in fp32 on the matrix cores.
+// GatedStaged, for the others, is on the 16-bit matrix cores: beside bf16 weights
+// x is cut into three bf16 planes whose sum is the value to 2^-24. Beside fp16 and
+// fp32 weights it is two fp16 planes, the value to 2^-23, after a power of two per
+// row that brings the row's largest magnitude to 2^14; fp32 weights are cut alike,
+// by rows, and for many rows bf16 ones become one fp16 plane, exact down to 2^-31
+// of the row's largest. Products x_i w_j but that of both second planes, smallest
+// first, fp32 sums: three matrix-core products a term for bf16 and fp32 weights, two
+// for fp16 and for bf16 as fp16. What fp16 planes leave out is below 2^-23 of
+// |x||w| a term and 2^-39 of the row's largest |x| times |w|; with fp32 weights
+// below 2^-21 at worst, for all of it, in the mean square some 2^-24, where a term
+// of fp32 arithmetic loses 2^-25 and the k fp32 sums that follow sqrt(k) 2^-25.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -39,6 +38,7 @@ typedef __attribute__((ext_vector_type(4))) short s16x4_t;
 typedef __attribute__((ext_vector_type(8))) short s16x8_t;
 
 constexpr int kStreamRows = 8;  // up to these: GatedStream
+constexpr int kMostSplits = 8;  // of a tile's steps
 
 constexpr int kRows = 16;   // rows of a panel, of x or a weight
 constexpr int kStep = 32;   // k of a step
@@ -163,8 +163,10 @@ __device__ __forceinline__ void ScalePanel(const GatedParams& p, int64_t which, 
 // x [m, k] into operand panels [panels][steps][planes][64 lanes][8]: zero past m
 // and k. A workgroup takes `chunk` steps of a panel, a wavefront a step at a time;
 // for planes of fp16 every workgroup of a panel first finds its rows' largest
-// magnitudes. Beside fp32 weights further workgroups find those of the weights'
-// columns.
+// magnitudes. Beside fp32 weights, and bf16 ones as fp16, further workgroups find
+// those of the weights' rows. Bound by bytes, small calls by latency: 2382 x 4096
+// 21 us (97 MB, 4.6 TB/s), 48 x 4096 5; with 2 x 16384 x 4096 bf16 weights 68 (365
+// MB, 5.4 TB/s), fp32 ones 102.
 template <int WT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void CutRows(GatedParams p, int chunk, int cuts) {
   constexpr int PL = Type<WT>::XPL;
@@ -284,8 +286,12 @@ __device__ __forceinline__ void LoadUnit(const Unit& u, unsigned char* buf, uint
 // planes and panel rows go from memory straight into LDS (buffer_load ... lds, 1
 // KiB units shared out over the wavefronts), NS - 1 steps
 // ahead. The weight is the A operand and x the B operand: a lane's four results
-// are four columns of one row of y. p.splits > 1: a workgroup takes a part of the
-// steps and leaves its sums, fragment by fragment, to GatedMerge.
+// are four columns of one row of y. Bound by the power the card may take at many
+// rows (bf16 as fp16, 2382 x 4096 x 16384, 1.28 PFLOP of products in 1100 us; three
+// bf16 planes 1.92 in 1313 at 1.7 GHz, where the matrix cores are busy 72% of the
+// cycles), by the panels' way through L2 at some hundred. p.splits > 1: a workgroup
+// takes a part of the steps and leaves its sums, fragment by fragment, to
+// GatedMerge.
 template <int WT, int WR, int WC, int XP, int WP, int NS, int ACT, int OCC>
 __global__ __launch_bounds__(64 * WR * WC) __attribute__((amdgpu_waves_per_eu(OCC)))
 void GatedStaged(GatedParams p) {
@@ -451,7 +457,7 @@ void GatedStaged(GatedParams p) {
   Fence();
   if constexpr (Type<WT>::kCols) {
 #pragma unroll
-    for (int b = 0; b < WP; ++b) asm volatile("" : "+v"(up[b]));  // waited for here, not in the loop
+    for (int b = 0; b < WP; ++b) asm volatile("" : "+v"(up[b]));  // waits here, not in the loop
   }
   int t = 0;
   auto step = [&](auto s) __attribute__((always_inline)) {
@@ -495,38 +501,42 @@ void GatedStaged(GatedParams p) {
 }
 
 // The split tiles of one row of wavefronts (WR = 1): their sums in split order,
-// then what the staged kernel does with whole ones. A workgroup a tile.
+// then what the staged kernel does with whole ones. A workgroup takes a panel of x
+// and, in each of a tile's wavefronts' parts, a gate and its up panel: few tiles
+// are split many ways, and their sums come from memory side by side (48 x 2048 x
+// 2048, 16 tiles in 8 parts, with a workgroup a tile 29.5 us in all).
 template <int WT, int WC, int XP, int WP, int ACT>
 __global__ __launch_bounds__(64 * WC) void GatedMerge(GatedParams p) {
   const int lane = threadIdx.x & 63, n16 = lane & 15, q = lane >> 4;
   const int wave = static_cast<int>(threadIdx.x >> 6);
-  const uint32_t tiles = static_cast<uint32_t>(p.row_tiles) * p.col_tiles, tile = blockIdx.x;
+  const uint32_t tiles = static_cast<uint32_t>(p.row_tiles) * p.col_tiles;
+  const uint32_t tile = blockIdx.x / (XP * (WP / 2)), rest = blockIdx.x - tile * (XP * (WP / 2));
+  const uint32_t a = rest / (WP / 2), b = rest - a * (WP / 2);
   // The staged kernel's order of tiles.
   const uint32_t band = tile / (4u * p.col_tiles);
   const uint32_t in_band = tile - band * 4u * p.col_tiles;
   const uint32_t h = min(4u, static_cast<uint32_t>(p.row_tiles) - 4u * band);
-  const int64_t xp0 = int64_t{4 * band + in_band % h} * XP;
-  const int64_t wp0 = int64_t{in_band / h} * (WC * WP / 2) + wave * WP / 2;
+  const int64_t row = (int64_t{4 * band + in_band % h} * XP + a) * kRows + n16;
+  const int64_t col = (int64_t{in_band / h} * (WC * WP / 2) + wave * WP / 2 + b) * kRows + 4 * q;
+  if (row >= p.m) return;
   const int64_t stride = int64_t{tiles} * WC * XP * WP * 64;
-  const f32x4_t* const from = reinterpret_cast<const f32x4_t*>(p.part) +
-                              (int64_t{tile} * WC + wave) * (XP * WP * 64) + lane;
+  const int64_t block = (int64_t{tile} * WC + wave) * (XP * WP) + a * WP + 2 * b;
+  const f32x4_t* const from = reinterpret_cast<const f32x4_t*>(p.part) + block * 64 + lane;
+  f32x4_t g[kMostSplits], u[kMostSplits];
 #pragma unroll
-  for (int a = 0; a < XP; ++a) {
-    const int64_t row = (xp0 + a) * kRows + n16;
-    if (row >= p.m) continue;
-    const int down = Type<WT>::kHalf ? p.row_scale[row] : 0;
-#pragma unroll
-    for (int b = 0; b < WP; b += 2) {
-      f32x4_t g = from[(a * WP + b) * 64], u = from[(a * WP + b + 1) * 64];
-      for (int i = 1; i < p.splits; ++i) {
-        g += from[i * stride + (a * WP + b) * 64];
-        u += from[i * stride + (a * WP + b + 1) * 64];
-      }
-      const int64_t col = (wp0 + b / 2) * kRows + 4 * q;
-      if constexpr (Type<WT>::kHalf) Rescale<Type<WT>::kCols>(p, col, down, &g, &u);
-      StoreRow4<false>(p, row, col, Finish<ACT>(p, col, g, u));
-    }
+  for (int i = 0; i < kMostSplits; ++i) {
+    const int64_t at = min(i, p.splits - 1) * stride;
+    g[i] = from[at];
+    u[i] = from[at + 64];
   }
+#pragma unroll
+  for (int i = 1; i < kMostSplits; ++i)
+    if (i < p.splits) {
+      g[0] += g[i];
+      u[0] += u[i];
+    }
+  if constexpr (Type<WT>::kHalf) Rescale<Type<WT>::kCols>(p, col, p.row_scale[row], &g[0], &u[0]);
+  StoreRow4<false>(p, row, col, Finish<ACT>(p, col, g[0], u[0]));
 }
 
 // Few rows (m <= MR): a workgroup per (panel, gate and up), its KW wavefronts
@@ -641,24 +651,36 @@ __global__ __launch_bounds__(64 * KW) void GatedStream(GatedParams p) {
   }
 }
 
-// fp32 weights and few rows or small sizes: a workgroup per (XP panels of x, gate
-// and up panel), on the fp32 matrix-core product of 16 x 16 x 4, whose operands
-// need no cutting: a lane's weights are single words of a panel's rows, and its x
-// four consecutive k of one row, in which product i of four takes the i-th. The
-// wavefronts take 16 k in turn and meet in LDS, in order. Its products cost five
-// times the planes', but there is no cutting and no pass over the weights before:
-// 40 x 4096 x 4096 39 us, of which the weights' bytes are 28, 100 rows 91 against
-// the staged kernel's 71 + 30 before it.
-template <int XP, int KW, int ACT>
+// Few rows or small sizes: a workgroup per (XP panels of x, gate and up panel), on
+// the fp32 matrix-core product of 16 x 16 x 4, whose operands need no cutting: a
+// lane's weights are single words of a panel's rows, and its x four consecutive k
+// of one row, in which product i of four takes the i-th. The wavefronts take 16 k in
+// turn and meet in LDS, in order. A product costs five times the planes' (16-bit
+// weights: eight to sixteen times), but there is one launch, no cutting and no pass
+// over the weights. Latency bounds it at few rows (bf16, 9 x 896 x 3584 7 us, 16 x
+// 4096 x 4096 18, of which the weights' bytes are 14), its products at more (fp32,
+// 40 x 4096 x 4096 39 us, of which the bytes are 28).
+template <int WT>
+__device__ __forceinline__ float Widen(typename Type<WT>::T v) {
+  if constexpr (WT == EHIP_WEIGHT_F32)
+    return v;
+  else if constexpr (WT == EHIP_WEIGHT_BF16)
+    return __uint_as_float(uint32_t{v} << 16);
+  else
+    return static_cast<float>(__builtin_bit_cast(_Float16, v));
+}
+
+template <int WT, int XP, int KW, int ACT>
 __global__ __launch_bounds__(64 * KW) void GatedDirect(GatedParams p) {
+  using T = typename Type<WT>::T;
   __shared__ f32x4_t red[KW][XP * 2][64];
   const int lane = threadIdx.x & 63, n16 = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const uint32_t xb = blockIdx.x / static_cast<uint32_t>(p.w_panels);
   const int64_t wp = blockIdx.x - xb * static_cast<uint32_t>(p.w_panels);
   const int64_t row0 = int64_t{xb} * XP * kRows + n16;
-  const float* const wg = static_cast<const float*>(p.wp[0]) + wp * p.k * kRows + n16;
-  const float* const wu = static_cast<const float*>(p.wp[1]) + wp * p.k * kRows + n16;
+  const T* const wg = static_cast<const T*>(p.wp[0]) + wp * p.k * kRows + n16;
+  const T* const wu = static_cast<const T*>(p.wp[1]) + wp * p.k * kRows + n16;
   f32x4_t acc[XP][2];
   const float* xr[XP];
 #pragma unroll
@@ -667,7 +689,8 @@ __global__ __launch_bounds__(64 * KW) void GatedDirect(GatedParams p) {
     // Rows past the last read the last one: their results are not stored.
     xr[a] = p.x + min(row0 + a * kRows, p.m - 1) * p.k;
   }
-  f32x4_t x[XP], w[2];
+  f32x4_t x[XP];
+  T w[2][4];  // as they are: widened where they are used, not where they are loaded
   auto load = [&](int64_t k0) __attribute__((always_inline)) {
     const int64_t kk = k0 + 4 * q;
     if (p.x_vec && k0 + 16 <= p.k) {
@@ -685,25 +708,30 @@ __global__ __launch_bounds__(64 * KW) void GatedDirect(GatedParams p) {
         const int64_t at = in ? kk + i : 0;
 #pragma unroll
         for (int a = 0; a < XP; ++a) x[a][i] = in ? xr[a][at] : 0.f;
-        w[0][i] = in ? wg[at * kRows] : 0.f;
-        w[1][i] = in ? wu[at * kRows] : 0.f;
+        w[0][i] = in ? wg[at * kRows] : T{};
+        w[1][i] = in ? wu[at * kRows] : T{};
       }
     }
   };
   int64_t k0 = int64_t{wave} * 16;
   if (k0 < p.k) load(k0);
   for (; k0 < p.k; k0 += 16 * KW) {
-    f32x4_t cx[XP], cw[2] = {w[0], w[1]};
+    f32x4_t cx[XP];
+    T cw[2][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) cw[0][i] = w[0][i], cw[1][i] = w[1][i];
 #pragma unroll
     for (int a = 0; a < XP; ++a) cx[a] = x[a];
     if (k0 + 16 * KW < p.k) load(k0 + 16 * KW);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i) {
+      const float v[2] = {Widen<WT>(cw[0][i]), Widen<WT>(cw[1][i])};
 #pragma unroll
       for (int a = 0; a < XP; ++a)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          acc[a][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(cw[h][i], cx[a][i], acc[a][h], 0, 0, 0);
+          acc[a][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[h], cx[a][i], acc[a][h], 0, 0, 0);
+    }
   }
 #pragma unroll
   for (int a = 0; a < XP; ++a)
@@ -722,14 +750,14 @@ __global__ __launch_bounds__(64 * KW) void GatedDirect(GatedParams p) {
   }
 }
 
-template <int XP, int ACT>
+template <int WT, int XP, int ACT>
 hipError_t LaunchDirect(const GatedParams& p, hipStream_t stream) {
   const int64_t n = (p.x_panels + XP - 1) / XP * p.w_panels;
-  if (n > INT32_MAX) return hipErrorInvalidValue;
+  if (n > UINT32_MAX / 512) return hipErrorInvalidValue;
   // Five panels' sums leave room for four wavefronts: 80 x 4096 x 4096 57 us, 65 with
   // eight; up to four panels eight are faster (128 rows 94 against 99).
   constexpr int kWaves = XP > 4 ? 4 : 8;
-  hipLaunchKernelGGL((GatedDirect<XP, kWaves, ACT>), dim3(static_cast<uint32_t>(n)),
+  hipLaunchKernelGGL((GatedDirect<WT, XP, kWaves, ACT>), dim3(static_cast<uint32_t>(n)),
                      dim3(64 * kWaves), 0, stream, p);
   return hipGetLastError();
 }
@@ -760,8 +788,9 @@ hipError_t LaunchTiles(GatedParams p, hipStream_t stream) {
   if constexpr (WR == 1 && WC == 4 && XP <= 4 && WP == 4) {  // the split tiles
     if (p.splits > 1) {
       if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-      hipLaunchKernelGGL((GatedMerge<WT, WC, XP, WP, ACT>), dim3(static_cast<uint32_t>(rt * ct)),
-                         dim3(64 * WC), 0, stream, p);
+      hipLaunchKernelGGL((GatedMerge<WT, WC, XP, WP, ACT>),
+                         dim3(static_cast<uint32_t>(rt * ct * XP * (WP / 2))), dim3(64 * WC), 0,
+                         stream, p);
     }
   }
   return hipGetLastError();
@@ -790,17 +819,15 @@ hipError_t Launch(const GatedParams& p, hipStream_t stream) {
   if (p.m <= 4) return LaunchStream<WT, 4, ACT>(p, stream);
   if (p.m <= kStreamRows) return LaunchStream<WT, 8, ACT>(p, stream);
   constexpr bool kF32 = WT == EHIP_WEIGHT_F32, kF16 = WT == EHIP_WEIGHT_F16;
-  if constexpr (kF32) {
-    if (p.tile == GatedTile::kDirect) {
-      // As few groups of rows as there can be, alike.
-      const int64_t groups = (p.x_panels + 4) / 5;
-      switch ((p.x_panels + groups - 1) / groups) {
-        case 1: return LaunchDirect<1, ACT>(p, stream);
-        case 2: return LaunchDirect<2, ACT>(p, stream);
-        case 3: return LaunchDirect<3, ACT>(p, stream);
-        case 4: return LaunchDirect<4, ACT>(p, stream);
-        default: return LaunchDirect<5, ACT>(p, stream);
-      }
+  if (p.tile == GatedTile::kDirect) {
+    // As few groups of rows as there can be, alike.
+    const int64_t groups = (p.x_panels + 4) / 5;
+    switch ((p.x_panels + groups - 1) / groups) {
+      case 1: return LaunchDirect<WT, 1, ACT>(p, stream);
+      case 2: return LaunchDirect<WT, 2, ACT>(p, stream);
+      case 3: return LaunchDirect<WT, 3, ACT>(p, stream);
+      case 4: return LaunchDirect<WT, 4, ACT>(p, stream);
+      default: return LaunchDirect<WT, 5, ACT>(p, stream);
     }
   }
   if constexpr (WT == EHIP_WEIGHT_BF16) {
@@ -860,17 +887,17 @@ hipError_t LaunchType(const GatedParams& p, hipStream_t stream) {
 // and no less than its bytes from L2 take at 9.6 TB/s. Where few rows leave CUs
 // idle, 16-bit weights: tiles of up to 64 x 128 whose steps are cut so that most
 // CUs have a part, 0.22 us a step and 0.09 for each panel of x, no less than 6.3
-// TB/s, and 6 us for the merge:
-//   16 x 4096 x 4096 25 of (43 at best whole), 48 rows 32 of (40), 16 x 4096 x 16384 53
-//   of (57); whole ones stay at 48 x 4096 x 16384, 64 of (64, split 66).
+// TB/s, and 3 us for the merge. Whole calls, bf16, split and at best whole: 48 x 4096
+// x 4096 23 and 35 us, 48 x 4096 x 16384 64 and 69, 17 x 2048 x 8192 21 and 25.
 // bf16 weights go as fp16 (their 8 bits fit, after a power of two per row) where
 // the third product costs more than a pass over them, 5.6 TB/s, and the
 // conversions: 2382 x 4096 x 16384 1100 + 68 of cutting and pass for 1313 + 21, 2382
 // x 4096 x 4096 327 + 36 for 379 + 21, 600 x 4096 x 16384 341 + 54 for 416 + 7.
-// fp32 weights leave GatedStaged where the cutting and the reading of the columns'
-// magnitudes that come before it (9 us and 5.2 TB/s) and its tiles take longer than
-// GatedDirect, 3.2 ns for a k of each panel of x that a CU has in turn: 100 x 4096 x
-// 4096 91 us direct and 101 staged, 200 x 896 x 3584 46 and 30.
+// A call leaves GatedStaged where what comes before it (8 us; fp32 weights 9 and the
+// reading of the columns' magnitudes at 5.2 TB/s) and its tiles take longer than
+// GatedDirect, 3.2 ns for a k of each panel of x that a CU has in turn. Whole calls,
+// direct and staged: fp32, 100 x 4096 x 4096 83 and 95 us, 200 x 896 x 3584 46 and 30;
+// bf16, 9 x 896 x 3584 7 and 14, 16 x 4096 x 4096 18 and 24, 40 x 896 x 3584 11 and 14.
 void PickTile(int weight_dtype, GatedParams* p) {
   struct Cost {
     GatedTile tile;
@@ -915,25 +942,27 @@ void PickTile(int weight_dtype, GatedParams* p) {
       return;
     }
   }
-  if (f32) {
-    const double words = static_cast<double>(p->w_panels * kRows) * static_cast<double>(p->k);
-    const int64_t groups = (p->x_panels + 4) / 5, panels = (p->x_panels + groups - 1) / groups;
-    const int64_t rounds = (groups * p->w_panels + p->cus - 1) / p->cus;
-    const double direct = 3.2e-3 * static_cast<double>(rounds * panels * p->k);
-    if (direct < least + 9 + 8 * words / 5.2e6) p->tile = GatedTile::kDirect;
-    return;
-  }
   const int64_t rows = std::min<int64_t>(p->x_panels, 4);
-  const int64_t splits = std::min<int64_t>({p->cus / tiles(rows, 8), p->steps / 8, 8});
-  if (splits < 2) return;
-  const int64_t part = (p->steps + splits - 1) / splits;
-  const double us = std::max(static_cast<double>(part) * (0.22 + 0.09 * static_cast<double>(rows)),
-                             traffic(rows, 8) / 6152) +
-                    6;
-  if (us >= least) return;
-  p->tile = GatedTile::kSplit;
-  p->split_steps = static_cast<int32_t>(part);
-  p->splits = static_cast<int32_t>((p->steps + part - 1) / part);
+  const int64_t splits = std::min<int64_t>({p->cus / tiles(rows, 8), p->steps / 8, kMostSplits});
+  const int64_t part = splits < 2 ? p->steps : (p->steps + splits - 1) / splits;
+  const double split_us =
+      std::max(static_cast<double>(part) * (0.22 + 0.09 * static_cast<double>(rows)),
+               traffic(rows, 8) / 6152) +
+      3;
+  if (!f32 && splits >= 2 && split_us < least) {
+    least = split_us;
+    p->tile = GatedTile::kSplit;
+    p->split_steps = static_cast<int32_t>(part);
+    p->splits = static_cast<int32_t>((p->steps + part - 1) / part);
+  }
+  const double words = static_cast<double>(p->w_panels * kRows) * static_cast<double>(p->k);
+  const int64_t groups = (p->x_panels + 4) / 5, panels = (p->x_panels + groups - 1) / groups;
+  const int64_t rounds = (groups * p->w_panels + p->cus - 1) / p->cus;
+  const double direct = 3.2e-3 * static_cast<double>(rounds * panels * p->k);
+  if (rounds < 32768 && direct < least + (f32 ? 9 + 8 * words / 5.2e6 : 8)) {
+    p->tile = GatedTile::kDirect;
+    p->splits = 1;
+  }
 }
 
 }  // namespace
