@@ -88,7 +88,11 @@ SHAPES = [(1, 1, 1), (1, 64, 16), (1, 896, 300), (2, 33, 17), (4, 4096, 96), (7,
           (130, 1030, 4096), (600, 1030, 1040), (600, 200, 2600), (700, 200, 4096),
           (1000, 96, 8000),
           # bf16 as fp16
-          (1300, 1001, 2600)]
+          (900, 513, 4100),
+          # the steps of tiles of one to four panels split
+          (13, 4097, 4100), (20, 3001, 70), (40, 2050, 70), (63, 2050, 70),
+          # tiles of 64 x 32 and 48 x 32
+          (257, 513, 1030), (70, 700, 70), (2400, 513, 129), (1500, 700, 272)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
@@ -154,7 +158,7 @@ def test_mxfp4_gated_against_64_bits(gctx, ehip_mod, m, k, n):
 
 
 @pytest.mark.parametrize("m,k,n", [(1, 128, 64), (8, 896, 100), (40, 64, 256), (300, 512, 256),
-                                   (600, 1024, 1040), (1300, 1024, 2600)])
+                                   (600, 1024, 1040), (900, 514, 4100)])
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 def test_every_plane_reaches_the_up_projection(gctx, ehip_mod, m, k, n, dtype):
     """With a zero gate weight and bias 64, act(64) = 64 exactly, so y = 64 u. x
@@ -227,12 +231,11 @@ def test_activations_over_their_range(gctx, ehip_mod, act):
         b.free()
 
 
-@pytest.mark.parametrize("m", [2, 20, 300])
+@pytest.mark.parametrize("m,k,n", [(2, 160, 100), (20, 160, 100), (600, 1030, 1040)])
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
-def test_non_finite_rows_stay_in_their_rows(gctx, ehip_mod, m, dtype):
+def test_non_finite_rows_stay_in_their_rows(gctx, ehip_mod, m, k, n, dtype):
     E = ehip_mod
     rng = np.random.default_rng(m)
-    k, n = 160, 100
     x = rng.standard_normal((m, k)).astype(np.float32)
     (gb, gv, code), (ub, uv, _) = (_weight(E, rng, n, k, dtype) for _ in range(2))
     x[1, 7], x[0, 159] = np.nan, np.inf
@@ -248,8 +251,8 @@ def test_non_finite_rows_stay_in_their_rows(gctx, ehip_mod, m, dtype):
         b.free()
 
 
-@pytest.mark.parametrize("m", [3, 20, 300])
-def test_fp16_subnormal_weights_and_rows_of_any_size(gctx, ehip_mod, m):
+@pytest.mark.parametrize("m,k,n", [(3, 200, 90), (20, 200, 90), (600, 1030, 1040)])
+def test_fp16_subnormal_weights_and_rows_of_any_size(gctx, ehip_mod, m, k, n):
     """Weights among fp16's subnormals (multiples of 2^-24) are exact; rows of x
     from 2^-120 to 2^100, one with a spike 2^20 times the rest, keep their
     precision: beside the module's bound the fp16 planes leave out 2^-39 of a
@@ -257,7 +260,6 @@ def test_fp16_subnormal_weights_and_rows_of_any_size(gctx, ehip_mod, m):
     weight, so y = 64 u."""
     E = ehip_mod
     rng = np.random.default_rng(m)
-    k, n = 200, 90
     x = rng.standard_normal((m, k))
     x[0, 5] *= 2.0**20
     x *= np.exp2(np.linspace(-120, 100, m))[:, None]
@@ -280,16 +282,16 @@ def test_fp16_subnormal_weights_and_rows_of_any_size(gctx, ehip_mod, m):
         b.free()
 
 
-@pytest.mark.parametrize("m", [3, 20, 70, 300])
+@pytest.mark.parametrize("m,k,n", [(3, 200, 90), (20, 200, 90), (70, 999, 129),
+                                   (600, 1030, 1040)])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-def test_bf16_planes_of_rows_of_any_size(gctx, ehip_mod, m, dtype):
+def test_planes_of_rows_of_any_size(gctx, ehip_mod, m, k, n, dtype):
     """Rows of x from 2^-120 to 2^100 keep their precision: beside the module's
     bound, planes below bf16's normal range may be lost, 2^-125 of |w| (of fp32
     weights too: of |x|) a term, and a sum's subnormals, 2^-126 an addition. y =
     64 u, as above."""
     E = ehip_mod
     rng = np.random.default_rng(m)
-    k, n = 200, 90
     x = rng.standard_normal((m, k)) * np.exp2(np.linspace(-120, 100, m))[:, None]
     x = x.astype(np.float32)
     (ub, uv, code), (gb, _, _) = (_weight(E, rng, n, k, dtype) for _ in range(2))
@@ -337,7 +339,7 @@ def test_mxfp4_passes_on_other_inputs_between(gctx, ehip_mod, m, k, n):
 
 @pytest.mark.parametrize("m,k,n,dtype", [(3, 200, 90, "f32"), (20, 200, 90, "f32"),
                                          (600, 1030, 1040, "f32"), (20, 200, 90, "bf16"),
-                                         (1300, 1030, 2600, "bf16")])
+                                         (900, 513, 4100, "bf16")])
 def test_weights_of_any_size(gctx, ehip_mod, m, k, n, dtype):
     """Rows of x from 2^-60 to 2^60 and weight rows from 2^-50 to 2^50, a spike
     2^20 times the rest in some of each, keep their precision: beside the module's
