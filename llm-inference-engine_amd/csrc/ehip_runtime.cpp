@@ -853,6 +853,13 @@ int CheckSizes(ehip_ctx* ctx, const char* what, int64_t m, int64_t k, int64_t n)
                   static_cast<long long>(n));
 }
 
+// How y's rows [.., n] can be stored: 2 in whole 128-byte lines, 1 in 16 bytes, 0 in
+// single words.
+int RowStores(int64_t n, const float* y) {
+  if (n % 32 == 0 && Aligned(y, 128)) return 2;
+  return n % 4 == 0 && Aligned(y, 16) ? 1 : 0;
+}
+
 int CheckActivation(ehip_ctx* ctx, const char* what, int32_t act) {
   if (act >= EHIP_ACT_SILU && act <= EHIP_ACT_GELU_TANH) return EHIP_OK;
   return SetError(ctx, EHIP_INVALID_ARGUMENT, "%s: activation=%d is not SILU/GELU/GELU_TANH", what,
@@ -896,7 +903,7 @@ int RunMxGemm(ehip_ctx* ctx, const float* x, const void* xc, const void* xs, int
   p.tiles = static_cast<int32_t>(ehip::MxTiles(k));
   p.groups = static_cast<int32_t>(ehip::MxGroups(k));
   p.x_vec = k % 4 == 0 && Aligned(x, 16);
-  p.y_vec = n % 4 == 0 && Aligned(d_y, 16);
+  p.y_vec = RowStores(n, d_y);
   p.act = act;
   EHIP_HIP(ctx, ehip::LaunchMxGemm(p, w.codes[1] != nullptr, ctx->stream));
   return EHIP_OK;
@@ -1029,7 +1036,7 @@ int ehip_packed_gated_gemm(ehip_ctx* ctx, const float* d_x, int64_t m, int64_t k
   p.col_scale = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(ctx->d_gemm) + p.col_at);
   p.part = reinterpret_cast<float*>(reinterpret_cast<char*>(ctx->d_gemm) + p.part_at);
   p.x_vec = k % 4 == 0 && Aligned(d_x, 16);
-  p.y_vec = n % 4 == 0 && Aligned(d_y, 16);
+  p.y_vec = RowStores(n, d_y);
   p.act = activation;
   EHIP_HIP(ctx, ehip::LaunchGatedGemm(p, weight_dtype, ctx->stream));
   return EHIP_OK;

@@ -536,7 +536,7 @@ __global__ __launch_bounds__(64 * WC) void GatedMerge(GatedParams p) {
       u[0] += u[i];
     }
   if constexpr (Type<WT>::kHalf) Rescale<Type<WT>::kCols>(p, col, p.row_scale[row], &g[0], &u[0]);
-  StoreRow4<false>(p, row, col, Finish<ACT>(p, col, g[0], u[0]));
+  StoreRow4<0>(p, row, col, Finish<ACT>(p, col, g[0], u[0]));
 }
 
 // Few rows (m <= MR): a workgroup per (panel, gate and up), its KW wavefronts
@@ -746,7 +746,7 @@ __global__ __launch_bounds__(64 * KW) void GatedDirect(GatedParams p) {
       for (int i = 1; i < KW; ++i) s[h] += red[i][2 * a + h][lane];
     }
     const int64_t col = wp * kRows + 4 * q;
-    StoreRow4<false>(p, row0 + a * kRows, col, Finish<ACT>(p, col, s[0], s[1]));
+    StoreRow4<0>(p, row0 + a * kRows, col, Finish<ACT>(p, col, s[0], s[1]));
   }
 }
 

@@ -257,7 +257,8 @@ struct GatedParams {
   int32_t splits, split_steps;
   // Where the row and column scales and the split sums begin (bytes).
   size_t scale_at, col_at, part_at;
-  int32_t x_vec, y_vec;  // rows are 16-byte aligned
+  int32_t x_vec;         // x's rows are 16-byte aligned
+  int32_t y_vec;         // y's: 1 16-byte aligned, 2 whole 128-byte lines, 0 neither
   int32_t act;           // EHIP_ACT_*
   int32_t row_tiles, col_tiles;  // the staged kernel's (set at its launch)
 };
@@ -293,7 +294,7 @@ struct MxGemmParams {
   int32_t tiles;          // 128-k tiles
   int32_t groups;         // scale groups of 4 tiles
   int32_t x_vec;          // x rows are 16-byte aligned
-  int32_t y_vec;          // y rows are 16-byte aligned
+  int32_t y_vec;          // y's: 1 16-byte aligned, 2 whole 128-byte lines, 0 neither
   int32_t act;            // EHIP_ACT_*
   int32_t row_tiles, col_tiles;  // the staged kernel's (set at its launch)
 };

@@ -352,7 +352,7 @@ __global__ __launch_bounds__(64 * KW) void MxDirect(MxGemmParams p) {
       for (int i = 1; i < KW; ++i) s[h] += red[i][f * PR + h][lane];
     }
     const int64_t col = wp * kMxRows + 4 * block;
-    StoreRow4<false>(p, (xp0 + f) * kMxRows + row, col, Finish<ACT>(p, col, s[0], s[PR - 1]));
+    StoreRow4<0>(p, (xp0 + f) * kMxRows + row, col, Finish<ACT>(p, col, s[0], s[PR - 1]));
   }
 }
 

@@ -50,17 +50,20 @@ __device__ __forceinline__ f32x4_t Finish(const P& p, int64_t col, f32x4_t g, f3
   return g;
 }
 
-// Four columns of a row of y, as far as they lie in it; STREAM: past the caches,
-// for the results of many rows. P has y, m, n, y_vec.
-template <bool STREAM, class P>
+// Four columns of a row of y, as far as they lie in it. P has y, m, n, y_vec.
+// STREAM: the least y_vec whose stores go past the caches (0: none's), for the
+// results of many rows: 1 where an instruction writes 128 bytes of a row and more,
+// 2 where it writes 64, which come together in L2 unless rows are whole lines (MXFP4
+// gated 2400 x 896 x 3584 23.7 us streamed and 25.3 cached, 2400 x 300 x 9000, whose
+// rows begin inside lines, 56 and 37; bf16, 128 bytes, 81 and 84).
+template <int STREAM, class P>
 __device__ __forceinline__ void StoreRow4(const P& p, int64_t row, int64_t col, const f32x4_t& v) {
   if (row >= p.m || col >= p.n) return;
   float* y = p.y + row * p.n + col;
-  if (p.y_vec) {  // n % 4 == 0
-    if constexpr (STREAM)
-      __builtin_nontemporal_store(v, reinterpret_cast<f32x4_t*>(y));
-    else
-      *reinterpret_cast<f32x4_t*>(y) = v;
+  if (STREAM > 0 && p.y_vec >= STREAM) {
+    __builtin_nontemporal_store(v, reinterpret_cast<f32x4_t*>(y));
+  } else if (p.y_vec) {  // n % 4 == 0
+    *reinterpret_cast<f32x4_t*>(y) = v;
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -133,7 +136,7 @@ __device__ __forceinline__ void StoreTile(const P& p, unsigned char* part, int64
       const int r = i * (64 / C) + lane / C, c = lane % C;
       const f32x4_t v =
           *reinterpret_cast<const f32x4_t*>(part + (r * C + ((c ^ r) & (C - 1))) * 16);
-      StoreRow4<true>(p, row0 + a0 * 16 + r, col0 + 4 * c, v);
+      StoreRow4<(C >= 8 ? 1 : 2)>(p, row0 + a0 * 16 + r, col0 + 4 * c, v);
     }
   }
 }
